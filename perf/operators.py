@@ -333,7 +333,7 @@ def _prepare_logits(c, rng, gen):
     if c["bias"]:
         counts = rng.randint(0, min(c["bias"], vocab) + 1, rows)
         counts[0] = min(c["bias"], vocab)
-        s["bias_tokens"] = _up(np.concatenate([rng.choice(vocab, n, replace=False) for n in counts]).astype(np.int32))
+        s["bias_tokens"] = _up(np.concatenate([np.sort(rng.choice(vocab, n, replace=False)) for n in counts]).astype(np.int32))
         s["bias_offsets"] = _up(np.concatenate([[0], np.cumsum(counts)]).astype(np.int32))
         s["bias_values"] = torch.randn(int(counts.sum()), generator=gen, device="cuda") * 4.0
     if c["masked"]:
@@ -355,6 +355,8 @@ def _prepare_logits(c, rng, gen):
                      "bias_tokens", "bias_values", "bias_offsets", "mask", "mask_rows"):
             if name in s:
                 setattr(d, name, s[name].data_ptr())
+        d.history_size = len(s["history"]) if c["penalties"] else 0
+        d.bias_size = len(s["bias_tokens"]) if c["bias"] else 0
         if c["masked"]:
             d.mask_stride, d.num_masks = s["mask"].shape[1], rows
         s.update(desc=d, call=kk.kernels()["logits_process"], kk=kk)
