@@ -211,6 +211,45 @@ KK_KAPI int kk_kv_write(const kk_kv_pools* pools, uint32_t layer_begin, uint32_t
 KK_KAPI int kk_kv_copy_tokens(const kk_kv_pools* pools, uint32_t layer_begin,
     uint32_t layer_count, const kk_kv_copy* copies, uint32_t num_copies, void* stream);
 
+/* Rotating append of a ragged batch (no counterpart in the reference, whose
+ * appends copy already rotated tokens, page_kernels.cu:77-127): one pass over
+ * `rows` token rows of any number of sequences rotates queries and keys to
+ * their positions and writes keys and values of one layer into the pages.
+ * Row r: pairs (d, d + rotary_dim/2) of every query and key head, d <
+ * rotary_dim/2, turn by positions[r] * theta^(-2d / rotary_dim); the other
+ * dims are copied. The angle is reduced in 64-bit fixed point and is off by
+ * less than 4e-6 rad at any 32-bit position; products are FP32, rounded once to
+ * FP16.
+ * A row whose slot is inactive is skipped: its query_out row and every page
+ * stay as they were. A slot outside its pool, or a position outside cos_sin's
+ * table, skips the row too and is reported by kk_device_status. Two active
+ * rows of one call must not name the same (slot, token).
+ * head_dim % 8 == 0, rotary_dim % 16 == 0, rotary_dim <= min(head_dim, 256);
+ * pointers 16-byte aligned (cos_sin: 8), strides multiples of 8 and not below
+ * the row they step over. query_out may be query itself (same stride). */
+typedef struct kk_kv_append_desc {
+    kk_kv_pools pools;
+    uint32_t layer;
+    uint32_t rows;              /* 0: nothing is launched */
+    uint32_t q_heads;           /* 0: no queries (query, query_out ignored) */
+    uint32_t rotary_dim;        /* 0: no rotation (theta, positions, cos_sin ignored) */
+    float theta;                /* >= 1 */
+    uint32_t table_positions;   /* rows of cos_sin */
+    const float* cos_sin;       /* optional [table_positions][rotary_dim / 2] pairs (cos, sin)
+                                   used in place of theta */
+    const kk_kv_slot* slots;    /* [rows] */
+    const uint32_t* positions;  /* [rows] */
+    const uint16_t* query;      /* [rows][q_heads][head_dim] at query_stride, and so on */
+    const uint16_t* key;
+    const uint16_t* value;
+    uint16_t* query_out;
+    uint64_t query_stride;
+    uint64_t key_stride;
+    uint64_t value_stride;
+    uint64_t query_out_stride;
+} kk_kv_append_desc;
+KK_KAPI int kk_kv_append_rope(const kk_kv_append_desc* desc, void* stream);
+
 /* Promotion copy: the 8 micro pages micro_slots[0..7] (all layers) become the
  * extent page extent_slot, tokens 8k..8k+7 <- micro page k (replaces
  * launchPromotion, src/cuda/kv/page_kernels.cu:129-182). */
@@ -335,6 +374,62 @@ KK_KAPI int kk_gemm_pack_weight_scaled(const uint16_t* weight, uint32_t M, uint3
 
 KK_KAPI uint64_t kk_argmax_workspace_bytes(uint32_t M, uint32_t N);
 KK_KAPI int kk_gemm(const kk_gemm_desc* desc, void* stream);
+
+/* ---- K7: penalties, biases and grammar masks on logits, greedy token -----------
+ * No counterpart in the reference (its LM head takes the argmax of the raw
+ * logits). Row r of FP32 logits x becomes, token by token, in this order:
+ *   1. v in the row's history (prompt or output), repetition p:
+ *        x = x > 0 ? x / p : x * p;
+ *   2. v given n >= 1 times in the output part of the history:
+ *        x = x - frequency * n, then x = x - presence;
+ *   3. v in the row's bias list: x = x + bias (of several entries for v the
+ *      last one counts);
+ *   4. v's mask bit clear: x = -inf, whatever x was (NaN included).
+ * Every operation is rounded to FP32 by itself. tokens[r] is the token of the
+ * highest logit, the lowest id among equals; NaN and -inf are never chosen, and
+ * a row that leaves nothing else gets KK_NO_TOKEN. Results do not depend on
+ * the order in which threads run.
+ * Strides are in elements; rows may start at any multiple of 4 bytes. vocab is
+ * at most 400,000 where a history or biases are given, 2^30 otherwise.
+ * Ids outside the vocabulary are ignored. Offsets that decrease or pass their
+ * array, bias ids that descend within a row and mask rows outside the masks are
+ * reported by kk_device_status; the row's history or biases are then left
+ * out, respectively the row is masked entirely. */
+#define KK_NO_TOKEN 0xffffffffu
+#define KK_NO_MASK 0xffffffffu
+typedef struct kk_logits_desc {
+    const float* logits;             /* [rows][vocab] at logits_stride */
+    float* out;                      /* may be logits itself (same stride); NULL: not written */
+    uint32_t* tokens;                /* [rows], or NULL */
+    uint64_t logits_stride;
+    uint64_t out_stride;
+    uint32_t rows;
+    uint32_t vocab;
+    /* Penalties: row r's token ids are history[history_offsets[r] .. [r + 1]),
+     * the first prompt_counts[r] of them the prompt (NULL: none). A NULL
+     * factor array is neutral (1, 0, 0); all three NULL: no history is read. */
+    const uint32_t* history;
+    const uint32_t* history_offsets; /* [rows + 1] */
+    const uint32_t* prompt_counts;   /* [rows] */
+    const float* repetition;         /* [rows] */
+    const float* presence;
+    const float* frequency;
+    uint64_t history_size;           /* entries of history */
+    /* Biases: row r's pairs are those at bias_offsets[r] .. [r + 1), ids
+     * ascending. NULL offsets: none. */
+    const uint32_t* bias_tokens;
+    const float* bias_values;
+    const uint32_t* bias_offsets;    /* [rows + 1] */
+    uint64_t bias_size;
+    /* Grammar masks: bit v % 32 of word v / 32 of a mask set: v is allowed.
+     * Row r uses mask mask_rows[r] (KK_NO_MASK: all allowed; NULL: mask r).
+     * NULL mask: none. */
+    const uint32_t* mask;            /* [num_masks] rows of mask_stride words */
+    const uint32_t* mask_rows;       /* [rows] */
+    uint32_t mask_stride;
+    uint32_t num_masks;
+} kk_logits_desc;
+KK_KAPI int kk_logits_process(const kk_logits_desc* desc, void* stream);
 
 /* Reads and clears the device-side status words of all kernel modules
  * (synchronises the stream). 0 = no kernel recorded an error. These words

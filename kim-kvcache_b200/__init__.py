@@ -379,6 +379,29 @@ class GemmDesc(C.Structure):
                 ("rope_cos_sin", C.c_void_p), ("rope_positions", C.c_uint32)]
 
 
+class KvAppendDesc(C.Structure):
+    _fields_ = [("pools", KvPools), ("layer", C.c_uint32), ("rows", C.c_uint32), ("q_heads", C.c_uint32),
+                ("rotary_dim", C.c_uint32), ("theta", C.c_float), ("table_positions", C.c_uint32),
+                ("cos_sin", C.c_void_p), ("slots", C.c_void_p), ("positions", C.c_void_p),
+                ("query", C.c_void_p), ("key", C.c_void_p), ("value", C.c_void_p),
+                ("query_out", C.c_void_p), ("query_stride", C.c_uint64), ("key_stride", C.c_uint64),
+                ("value_stride", C.c_uint64), ("query_out_stride", C.c_uint64)]
+
+
+NO_TOKEN = NO_MASK = 0xFFFFFFFF
+
+
+class LogitsDesc(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("out", C.c_void_p), ("tokens", C.c_void_p),
+                ("logits_stride", C.c_uint64), ("out_stride", C.c_uint64), ("rows", C.c_uint32),
+                ("vocab", C.c_uint32), ("history", C.c_void_p), ("history_offsets", C.c_void_p),
+                ("prompt_counts", C.c_void_p), ("repetition", C.c_void_p), ("presence", C.c_void_p),
+                ("frequency", C.c_void_p), ("history_size", C.c_uint64), ("bias_tokens", C.c_void_p),
+                ("bias_values", C.c_void_p), ("bias_offsets", C.c_void_p), ("bias_size", C.c_uint64),
+                ("mask", C.c_void_p), ("mask_rows", C.c_void_p), ("mask_stride", C.c_uint32),
+                ("num_masks", C.c_uint32)]
+
+
 _VP = C.c_void_p
 KERNEL_SIGNATURES = {
     "attention_plan": (_U32, [C.POINTER(PageDesc), C.POINTER(AttnLane), _U32, _U32,
@@ -403,6 +426,8 @@ KERNEL_SIGNATURES = {
     "gemm_packed_bytes": (_U64, [_U32, _U32]),
     "gemm_pack_weight": (_I, [_VP, _U32, _U32, _VP, _VP]),
     "gemm_pack_weight_scaled": (_I, [_VP, _U32, _U32, _VP, _VP, _VP]),
+    "kv_append_rope": (_I, [C.POINTER(KvAppendDesc), _VP]),
+    "logits_process": (_I, [C.POINTER(LogitsDesc), _VP]),
     "kv_promote": (_I, [C.POINTER(KvPools), C.POINTER(_U32), _U32, _VP]),
     "kv_gather": (_I, [C.POINTER(KvPools), _VP, _U32, _U32, _VP, _VP]),
     "kv_scatter": (_I, [C.POINTER(KvPools), _VP, _U32, _U32, _U32, _VP, _VP]),

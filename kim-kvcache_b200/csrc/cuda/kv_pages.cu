@@ -12,6 +12,8 @@
 #include "kernels_internal.h"
 #include "launch.cuh"
 
+#include <cmath>
+
 namespace kk {
 
 __device__ unsigned int g_pages_status;
@@ -120,6 +122,199 @@ __global__ void kv_copy_kernel(PoolView v, std::uint32_t layer_begin, kk_kv_copy
     std::uint64_t const n = std::uint64_t(c.tokens) * v.row;
     for (std::uint64_t i = threadIdx.x * 8u; i < n; i += blockDim.x * 8u) {
         *reinterpret_cast<uint4*>(dst + i) = *reinterpret_cast<uint4 const*>(src + i);
+    }
+}
+
+// ---- kk_kv_append_rope --------------------------------------------------------
+
+constexpr std::uint32_t kMaxRotaryDim = 256;
+constexpr int kAppendThreads = 256;
+constexpr std::uint32_t kAppendMaxRows = 8;  // rows per CTA, at most
+
+struct AppendArgs {
+    PoolView pools;
+    std::uint32_t layer;
+    std::uint32_t rows;
+    std::uint32_t rows_per_cta;
+    std::uint32_t q_heads;
+    std::uint32_t kv_heads;
+    std::uint32_t head_dim;
+    std::uint32_t rotary_half;
+    std::uint32_t table_positions;
+    float2 const* cos_sin;
+    kk_kv_slot const* slots;
+    std::uint32_t const* positions;
+    __half const* query;
+    __half const* key;
+    __half const* value;
+    __half* query_out;
+    std::uint64_t query_stride;
+    std::uint64_t key_stride;
+    std::uint64_t value_stride;
+    std::uint64_t query_out_stride;
+    // theta^(-2d / rotary_dim) / (2 pi) turns per position, as 0.64 fixed point.
+    std::uint64_t turns[kMaxRotaryDim / 2];
+};
+
+// Rotates queries and keys of rows_per_cta token rows per CTA and writes keys
+// and values into their pages. A byte mover: every input element is read once
+// and every output written once, 16 bytes at a time, so HBM bounds it. A step
+// is 8 pairs (16 + 16 bytes) of one rotated head, or 8 copied elements. The
+// (cos, sin) of a row are computed once for all of its heads and kept in shared
+// memory; a thread's first steps are requested before them, so that the loads
+// run under that arithmetic. Angles: position * turns in 64-bit fixed point
+// drops whole turns exactly, and the top 32 bits of what is left are the
+// angle to 2^-32 turns at any position.
+__global__ void __launch_bounds__(kAppendThreads) kv_append_rope_kernel(const __grid_constant__ AppendArgs a)
+{
+    __shared__ float2 s_cs[kAppendMaxRows * (kMaxRotaryDim / 2)];  // [row][pair]
+    __shared__ __half* s_dst[kAppendMaxRows];  // key of the row's token in its page; null: row skipped
+    __shared__ std::uint32_t s_value[kAppendMaxRows];  // elements from there to its value
+    pdl_launch_dependents();
+    pdl_wait();
+    std::uint32_t const row0 = blockIdx.x * a.rows_per_cta;
+    std::uint32_t const left = a.rows - row0;
+    std::uint32_t const n_rows = left < a.rows_per_cta ? left : a.rows_per_cta;
+    std::uint32_t const tid = threadIdx.x;
+    std::uint32_t const half = a.rotary_half;
+    std::uint32_t const chunks = half / 8u;                   // steps per rotated head
+    std::uint32_t const row_steps = (a.q_heads + a.kv_heads) * chunks;
+    std::uint32_t const steps = n_rows * row_steps;
+    std::uint32_t const row_copies = a.pools.row / 8u;
+    std::uint32_t const copies = n_rows * row_copies;
+
+    struct Step {
+        std::uint32_t row;   // within the CTA
+        std::uint32_t head;  // queries first, then keys
+        std::uint32_t pair;  // first of its 8 pairs
+    };
+    auto locate = [&](std::uint32_t i) {
+        std::uint32_t const row = i / row_steps;
+        std::uint32_t const rest = i - row * row_steps;
+        std::uint32_t const head = rest / chunks;
+        return Step{row, head, (rest - head * chunks) * 8u};
+    };
+    auto source = [&](Step const& s) {
+        std::uint64_t const row = row0 + s.row;
+        return (s.head < a.q_heads ? a.query + row * a.query_stride + s.head * a.head_dim
+                                   : a.key + row * a.key_stride + (s.head - a.q_heads) * a.head_dim) + s.pair;
+    };
+    auto value_source = [&](std::uint32_t i) {
+        std::uint32_t const row = i / row_copies;
+        return a.value + (row0 + row) * a.value_stride + (i - row * row_copies) * 8u;
+    };
+
+    Step cur{};
+    uint4 lo{}, hi{}, val{};
+    if (tid < steps) {
+        cur = locate(tid);
+        __half const* src = source(cur);
+        lo = *reinterpret_cast<uint4 const*>(src);
+        hi = *reinterpret_cast<uint4 const*>(src + half);
+    }
+    if (tid < copies) {
+        val = *reinterpret_cast<uint4 const*>(value_source(tid));
+    }
+
+    if (tid < n_rows) {
+        kk_kv_slot const slot = a.slots[row0 + tid];
+        __half* dst = nullptr;
+        std::uint32_t const cap = slot.kind == 0 ? a.pools.micro_cap : 64u;
+        if (slot.active) {
+            if (slot.page_token >= cap || slot.kind > 1u) {
+                report(a.pools, kErrBadDescriptor);
+            } else if (a.cos_sin != nullptr && a.positions[row0 + tid] >= a.table_positions) {
+                report(a.pools, kErrBadArgument);
+            } else {
+                dst = block_of(a.pools, slot.kind, slot.slot, a.layer, 0);
+                if (dst != nullptr) {
+                    dst += std::uint64_t(slot.page_token) * a.pools.row;
+                }
+            }
+        }
+        s_dst[tid] = dst;
+        s_value[tid] = cap * a.pools.row;
+    }
+    for (std::uint32_t i = tid; i < n_rows * half; i += kAppendThreads) {
+        std::uint32_t const row = i / half;
+        std::uint32_t const d = i - row * half;
+        std::uint32_t const position = a.positions[row0 + row];
+        float2 cs;
+        if (a.cos_sin != nullptr) {
+            cs = position < a.table_positions ? a.cos_sin[std::uint64_t(position) * half + d] : make_float2(1.f, 0.f);
+        } else {
+            std::uint64_t const turn = position * a.turns[d];  // modulo one turn
+            // Half turns in [-1, 1).
+            sincospif(static_cast<float>(static_cast<std::int32_t>(turn >> 32)) * 0x1p-31f, &cs.y, &cs.x);
+        }
+        s_cs[i] = cs;
+    }
+    __syncthreads();
+
+    for (std::uint32_t i = tid; i < steps;) {
+        std::uint32_t const next = i + kAppendThreads;
+        Step const s = cur;
+        uint4 const xa = lo, xb = hi;
+        if (next < steps) {
+            cur = locate(next);
+            __half const* src = source(cur);
+            lo = *reinterpret_cast<uint4 const*>(src);
+            hi = *reinterpret_cast<uint4 const*>(src + half);
+        }
+        i = next;
+        __half* dst = s_dst[s.row];
+        if (dst == nullptr) {
+            continue;
+        }
+        __half2 const* pa = reinterpret_cast<__half2 const*>(&xa);
+        __half2 const* pb = reinterpret_cast<__half2 const*>(&xb);
+        float4 const* cs = reinterpret_cast<float4 const*>(&s_cs[s.row * half + s.pair]);
+        uint4 ya, yb;
+        __half2* qa = reinterpret_cast<__half2*>(&ya);
+        __half2* qb = reinterpret_cast<__half2*>(&yb);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float2 const fa = __half22float2(pa[e]);
+            float2 const fb = __half22float2(pb[e]);
+            float4 const c = cs[e];  // (cos, sin) of two pairs
+            qa[e] = __floats2half2_rn(fa.x * c.x - fb.x * c.y, fa.y * c.z - fb.y * c.w);
+            qb[e] = __floats2half2_rn(fb.x * c.x + fa.x * c.y, fb.y * c.z + fa.y * c.w);
+        }
+        dst = s.head < a.q_heads
+            ? a.query_out + (row0 + s.row) * a.query_out_stride + s.head * a.head_dim + s.pair
+            : dst + (s.head - a.q_heads) * a.head_dim + s.pair;
+        *reinterpret_cast<uint4*>(dst) = ya;
+        *reinterpret_cast<uint4*>(dst + half) = yb;
+    }
+    for (std::uint32_t i = tid; i < copies;) {
+        std::uint32_t const row = i / row_copies;
+        std::uint32_t const e = (i - row * row_copies) * 8u;
+        uint4 const x = val;
+        i += kAppendThreads;
+        if (i < copies) {
+            val = *reinterpret_cast<uint4 const*>(value_source(i));
+        }
+        __half* dst = s_dst[row];
+        if (dst != nullptr) {
+            *reinterpret_cast<uint4*>(dst + s_value[row] + e) = x;
+        }
+    }
+    // Dims behind the rotated ones.
+    std::uint32_t const tail = a.head_dim - 2u * half;
+    std::uint32_t const head_copies = tail / 8u;
+    std::uint32_t const row_tails = (a.q_heads + a.kv_heads) * head_copies;
+    for (std::uint32_t i = tid; i < n_rows * row_tails; i += kAppendThreads) {
+        std::uint32_t const row = i / row_tails;
+        std::uint32_t const rest = i - row * row_tails;
+        std::uint32_t const head = rest / head_copies;
+        std::uint32_t const e = 2u * half + (rest - head * head_copies) * 8u;
+        __half* dst = s_dst[row];
+        if (dst == nullptr) {
+            continue;
+        }
+        dst = head < a.q_heads ? a.query_out + (row0 + row) * a.query_out_stride + head * a.head_dim + e
+                               : dst + (head - a.q_heads) * a.head_dim + e;
+        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4 const*>(source(Step{row, head, e}));
     }
 }
 
@@ -238,6 +433,79 @@ int kk_kv_copy_tokens(const kk_kv_pools* pools, uint32_t layer_begin, uint32_t l
 {
     return kk::kvCopy(pools, layer_begin, layer_count, copies, num_copies, nullptr,
         static_cast<cudaStream_t>(stream));
+}
+
+int kk_kv_append_rope(const kk_kv_append_desc* d, void* stream)
+{
+    using namespace kk;
+    auto misaligned = [](void const* p, std::uint64_t stride, std::uint64_t row) {
+        return p == nullptr || (reinterpret_cast<std::uintptr_t>(p) & 15u) != 0 || stride % 8 != 0 || stride < row;
+    };
+    if (d == nullptr || !poolsOk(&d->pools) || d->layer >= d->pools.layers || d->pools.head_dim % 8 != 0
+        || (reinterpret_cast<std::uintptr_t>(d->pools.micro) & 15u) != 0
+        || (reinterpret_cast<std::uintptr_t>(d->pools.extent) & 15u) != 0
+        || d->rotary_dim % 16 != 0 || d->rotary_dim > d->pools.head_dim || d->rotary_dim > kMaxRotaryDim) {
+        return KK_EINVAL;
+    }
+    // Heads and dims that cannot be counted in 32-bit steps are no model's.
+    std::uint64_t const q_row = std::uint64_t(d->q_heads) * d->pools.head_dim;
+    std::uint64_t const kv_row = std::uint64_t(d->pools.kv_heads) * d->pools.head_dim;
+    if (q_row > (1u << 24) || kv_row > (1u << 24)) {
+        return KK_EINVAL;
+    }
+    if (d->rows == 0) {
+        return 0;
+    }
+    if (d->slots == nullptr || misaligned(d->key, d->key_stride, kv_row)
+        || misaligned(d->value, d->value_stride, kv_row)
+        || (d->q_heads != 0
+            && (misaligned(d->query, d->query_stride, q_row) || misaligned(d->query_out, d->query_out_stride, q_row)
+                || (d->query == d->query_out && d->query_stride != d->query_out_stride)))) {
+        return KK_EINVAL;
+    }
+    AppendArgs a{};
+    if (d->rotary_dim != 0) {
+        if (d->positions == nullptr || (reinterpret_cast<std::uintptr_t>(d->cos_sin) & 7u) != 0
+            || (d->cos_sin != nullptr && d->table_positions == 0)
+            || (d->cos_sin == nullptr && !(d->theta >= 1.f && std::isfinite(d->theta)))) {
+            return KK_EINVAL;
+        }
+        a.cos_sin = reinterpret_cast<float2 const*>(d->cos_sin);
+        a.table_positions = d->table_positions;
+        if (a.cos_sin == nullptr) {
+            // theta^(-2i / rotary_dim) by repeated products of one power. The
+            // i-th is off by i roundings of 2^-53 of a value that shrinks
+            // with i: below 2^-53 turns per position, 2^-21 at the farthest.
+            double const ratio = std::pow(static_cast<double>(d->theta), -2.0 / d->rotary_dim);
+            double turns = 0.15915494309189535;  // 1 / (2 pi)
+            for (std::uint32_t i = 0; i < d->rotary_dim / 2; ++i, turns *= ratio) {
+                a.turns[i] = static_cast<std::uint64_t>((turns - std::floor(turns)) * 0x1p64);
+            }
+        }
+    }
+    a.pools = view(d->pools);
+    a.layer = d->layer;
+    a.rows = d->rows;
+    // Few rows: one CTA each, for the shortest chain of loads. Many: enough
+    // rows per CTA that its threads take several steps each.
+    a.rows_per_cta = d->rows <= 1024u ? 1u : 4u;
+    a.q_heads = d->q_heads;
+    a.kv_heads = d->pools.kv_heads;
+    a.head_dim = d->pools.head_dim;
+    a.rotary_half = d->rotary_dim / 2;
+    a.slots = d->slots;
+    a.positions = d->positions;
+    a.query = reinterpret_cast<__half const*>(d->query);
+    a.key = reinterpret_cast<__half const*>(d->key);
+    a.value = reinterpret_cast<__half const*>(d->value);
+    a.query_out = reinterpret_cast<__half*>(d->query_out);
+    a.query_stride = d->query_stride;
+    a.key_stride = d->key_stride;
+    a.value_stride = d->value_stride;
+    a.query_out_stride = d->query_out_stride;
+    unsigned const grid = (d->rows + a.rows_per_cta - 1u) / a.rows_per_cta;
+    return static_cast<int>(launch(kv_append_rope_kernel, dim3(grid), dim3(kAppendThreads), 0,
+        static_cast<cudaStream_t>(stream), 1, a));
 }
 
 int kk_kv_promote(const kk_kv_pools* pools, const uint32_t* micro_slots, uint32_t extent_slot,

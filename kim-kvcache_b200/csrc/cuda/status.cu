@@ -29,6 +29,7 @@ int attentionStatus(cudaStream_t stream);
 int attentionTmaStatus(cudaStream_t stream);
 int pagesStatus(cudaStream_t stream);
 int gemmStatus(cudaStream_t stream);
+int logitsStatus(cudaStream_t stream);
 
 } // namespace kk
 
@@ -37,8 +38,8 @@ extern "C" {
 int kk_device_status(void* stream)
 {
     cudaStream_t const s = static_cast<cudaStream_t>(stream);
-    int const codes[4] = {kk::attentionStatus(s), kk::attentionTmaStatus(s), kk::pagesStatus(s),
-        kk::gemmStatus(s)};
+    int const codes[] = {kk::attentionStatus(s), kk::attentionTmaStatus(s), kk::pagesStatus(s),
+        kk::gemmStatus(s), kk::logitsStatus(s)};
     for (int c : codes) {
         if (c != 0) {
             return c;
