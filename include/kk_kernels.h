@@ -197,6 +197,103 @@ KK_KAPI int kk_paged_decode_attention_noalloc(const kk_kv_pools* pools, uint32_t
 #define KK_ATTN_TMA 2
 KK_KAPI int kk_attention_set_variant(int variant);
 
+/* ---- K8: decode attention of lanes that share a prefix ----------------------------
+ * No counterpart in the reference, whose forks each read the shared pages
+ * (paged_decode_kernels.cu:533-617 walks every lane's whole table). Lanes whose
+ * block tables begin with the same pages (forks of one prompt, the positions
+ * of one prompt chunk) form a group; the group's pages are read once for all of
+ * its query rows, each lane's remaining pages for that lane alone, and the
+ * softmax parts are joined exactly. Same results as kk_paged_decode_attention
+ * over the whole tables, up to FP32 rounding of the softmax sums.
+ *
+ * Host side, once per step (the plan serves every layer):
+ *   kk_prefix_groups finds the groups and cuts the shared pages off the lanes'
+ *   tables; kk_prefix_attention_plan makes the work list; descriptors, lanes,
+ *   groups and items are copied to the device.
+ * head_dim must be 64; q_heads / kv_heads <= 16. */
+typedef struct kk_prefix_group {
+    uint32_t desc_offset;      /* the shared pages' descriptors */
+    uint32_t desc_count;
+    uint32_t token_count;
+    uint32_t lane_begin;       /* lanes [lane_begin, lane_begin + lane_count) share them */
+    uint32_t lane_count;
+    uint32_t part_row;         /* filled by the plan: first partial row, */
+    uint32_t part_count;       /* splits of the prefix, */
+    uint32_t row_tiles;        /* tiles of 128 query rows per KV head */
+} kk_prefix_group;
+
+typedef struct kk_prefix_item {
+    uint32_t owner;            /* group (row_tiles != 0) or lane (row_tiles == 0) */
+    uint32_t kv_head;
+    uint32_t desc_begin;       /* run of the descriptor array */
+    uint32_t desc_end;
+    uint32_t part;
+    uint16_t row_tile;         /* first tile of query rows */
+    uint16_t row_tiles;        /* 1 or 2; 0: a lane's own pages */
+    uint32_t token_tiles;      /* 128-token tiles of the run */
+    uint32_t reserved;
+} kk_prefix_item;
+
+typedef struct kk_prefix_plan {
+    uint32_t num_items;        /* shared items first, then lanes' own */
+    uint32_t num_shared;
+    uint32_t tasks_per_cta;    /* lanes' own items per thread block */
+    uint32_t num_lanes;
+    uint32_t num_groups;
+    uint32_t num_descs;
+    uint32_t q_heads;
+    uint32_t kv_heads;
+    uint64_t part_rows;        /* partial softmax rows in the workspace */
+} kk_prefix_plan;
+
+/* Finds runs of at least max(2, min_lanes) consecutive lanes whose tables
+ * begin with the same pages (slot, kind and valid tokens) for at least
+ * min_tokens tokens, writes a group for each and moves the shared descriptors
+ * out of those lanes (desc_offset, desc_count, token_count). A group takes
+ * the pages that its first two lanes share, and the lanes that share all of
+ * them. Returns the groups written (<= max_groups). */
+KK_KAPI uint32_t kk_prefix_groups(const kk_page_desc* host_descs, kk_attn_lane* host_lanes,
+    uint32_t num_lanes, uint32_t min_lanes, uint32_t min_tokens, kk_prefix_group* host_groups,
+    uint32_t max_groups);
+/* Splits the groups' pages and the lanes' own pages into items for num_sms
+ * SMs. Fills item_offset, item_count and reserved (1 + group, 0: none) of
+ * every lane, the part fields of every group, the items (those beyond
+ * max_items are counted, not written) and the plan. Groups may come from
+ * kk_prefix_groups or be made by the caller; a lane belongs to one group at
+ * most. KK_EINVAL: a range outside its array, a lane in two groups, head
+ * counts that are not served, or more than 2^32 - 1 partial rows. */
+KK_KAPI int kk_prefix_attention_plan(const kk_page_desc* host_descs, uint32_t num_descs,
+    kk_attn_lane* host_lanes, uint32_t num_lanes, kk_prefix_group* host_groups, uint32_t num_groups,
+    uint32_t q_heads, uint32_t kv_heads, uint32_t num_sms, kk_prefix_item* host_items,
+    uint32_t max_items, kk_prefix_plan* plan);
+/* Workspace of a call (16-byte aligned, no initial values). Calls that can
+ * overlap need one each. */
+KK_KAPI uint64_t kk_prefix_attention_workspace_bytes(const kk_prefix_plan* plan);
+
+typedef struct kk_prefix_attn_desc {
+    kk_kv_pools pools;
+    uint32_t layer;
+    uint32_t q_heads;
+    float scale;
+    uint32_t reserved;
+    kk_prefix_plan plan;
+    const kk_page_desc* descs;      /* device copies of the plan's arrays */
+    const kk_attn_lane* lanes;
+    const kk_prefix_group* groups;
+    const kk_prefix_item* items;
+    const uint16_t* query;          /* rows lane.query_row: [q_heads][64] at query_stride */
+    uint16_t* output;
+    uint64_t query_stride;
+    uint64_t output_stride;
+    void* workspace;
+    uint64_t workspace_bytes;
+} kk_prefix_attn_desc;
+/* A lane that has no tokens at all gets zeros. Descriptors outside their pool
+ * or over their page contribute nothing and are reported by kk_device_status,
+ * as are items that do not fit the plan. query and output are 16-byte aligned,
+ * strides multiples of 8. */
+KK_KAPI int kk_prefix_attention(const kk_prefix_attn_desc* desc, void* stream);
+
 /* ---- K2: batched KV append / copy-on-write -----------------------------------
  * kk_kv_write replaces launchWriteLayerToken (paged_decode_kernels.cu:65-99) and
  * launchAppendTokens (src/cuda/kv/page_kernels.cu:77-127) for one token per

@@ -388,6 +388,32 @@ class KvAppendDesc(C.Structure):
                 ("value_stride", C.c_uint64), ("query_out_stride", C.c_uint64)]
 
 
+class PrefixGroup(C.Structure):
+    _fields_ = [("desc_offset", C.c_uint32), ("desc_count", C.c_uint32), ("token_count", C.c_uint32),
+                ("lane_begin", C.c_uint32), ("lane_count", C.c_uint32), ("part_row", C.c_uint32),
+                ("part_count", C.c_uint32), ("row_tiles", C.c_uint32)]
+
+
+class PrefixItem(C.Structure):
+    _fields_ = [("owner", C.c_uint32), ("kv_head", C.c_uint32), ("desc_begin", C.c_uint32),
+                ("desc_end", C.c_uint32), ("part", C.c_uint32), ("row_tile", C.c_uint16),
+                ("row_tiles", C.c_uint16), ("token_tiles", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+class PrefixPlan(C.Structure):
+    _fields_ = [("num_items", C.c_uint32), ("num_shared", C.c_uint32), ("tasks_per_cta", C.c_uint32),
+                ("num_lanes", C.c_uint32), ("num_groups", C.c_uint32), ("num_descs", C.c_uint32),
+                ("q_heads", C.c_uint32), ("kv_heads", C.c_uint32), ("part_rows", C.c_uint64)]
+
+
+class PrefixAttnDesc(C.Structure):
+    _fields_ = [("pools", KvPools), ("layer", C.c_uint32), ("q_heads", C.c_uint32), ("scale", C.c_float),
+                ("reserved", C.c_uint32), ("plan", PrefixPlan), ("descs", C.c_void_p),
+                ("lanes", C.c_void_p), ("groups", C.c_void_p), ("items", C.c_void_p),
+                ("query", C.c_void_p), ("output", C.c_void_p), ("query_stride", C.c_uint64),
+                ("output_stride", C.c_uint64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
+
+
 NO_TOKEN = NO_MASK = 0xFFFFFFFF
 
 
@@ -426,6 +452,13 @@ KERNEL_SIGNATURES = {
     "gemm_packed_bytes": (_U64, [_U32, _U32]),
     "gemm_pack_weight": (_I, [_VP, _U32, _U32, _VP, _VP]),
     "gemm_pack_weight_scaled": (_I, [_VP, _U32, _U32, _VP, _VP, _VP]),
+    "prefix_groups": (_U32, [C.POINTER(PageDesc), C.POINTER(AttnLane), _U32, _U32, _U32,
+                             C.POINTER(PrefixGroup), _U32]),
+    "prefix_attention_plan": (_I, [C.POINTER(PageDesc), _U32, C.POINTER(AttnLane), _U32,
+                                   C.POINTER(PrefixGroup), _U32, _U32, _U32, _U32, C.POINTER(PrefixItem),
+                                   _U32, C.POINTER(PrefixPlan)]),
+    "prefix_attention_workspace_bytes": (_U64, [C.POINTER(PrefixPlan)]),
+    "prefix_attention": (_I, [C.POINTER(PrefixAttnDesc), _VP]),
     "kv_append_rope": (_I, [C.POINTER(KvAppendDesc), _VP]),
     "logits_process": (_I, [C.POINTER(LogitsDesc), _VP]),
     "kv_promote": (_I, [C.POINTER(KvPools), C.POINTER(_U32), _U32, _VP]),

@@ -1222,6 +1222,12 @@ int smCount()
 
 } // namespace
 
+bool encodePageHeadMap(CUtensorMap* map, void const* base, std::uint32_t pages, std::uint32_t cap,
+    std::uint32_t layers, std::uint32_t heads, std::uint32_t box_tokens)
+{
+    return encodePerHead(map, base, pages, cap, layers, heads, box_tokens);
+}
+
 bool attentionTmaSupported(kk_kv_pools const* pools, std::uint32_t q_heads)
 {
     return pools != nullptr && pools->head_dim == kHeadDim && pools->micro != nullptr

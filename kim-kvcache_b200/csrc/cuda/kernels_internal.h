@@ -6,6 +6,7 @@
 
 #include "../../../include/kk_kernels.h"
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -74,6 +75,12 @@ int attentionTmaLaunch(kk_kv_pools const* pools, std::uint32_t layer, std::uint3
     std::uint16_t const* query, std::uint32_t query_stride, std::uint16_t* output,
     std::uint32_t output_stride, float scale, std::uint32_t* counters, float* part_o, float* part_ml,
     unsigned int* status, cudaStream_t stream);
+
+// Tensor map of a pool of `cap`-token pages, [page][layer*2+kv][token][kv_head]
+// [64 dims] FP16, whose box is `box_tokens` tokens of one head (128-byte
+// swizzle). False when the driver refuses it.
+bool encodePageHeadMap(CUtensorMap* map, void const* base, std::uint32_t pages, std::uint32_t cap,
+    std::uint32_t layers, std::uint32_t heads, std::uint32_t box_tokens);
 
 // kk_kv_copy_tokens with the copy count in device memory (<= max_copies).
 int kvCopyDevCount(kk_kv_pools const* pools, std::uint32_t layer_begin, std::uint32_t layer_count,

@@ -1,0 +1,1435 @@
+// K8 — decode attention of lanes that share a prefix, for sm_100a.
+//
+// Lanes of a group see the same leading pages. Their query rows of one KV head
+// (lane_count x query heads per KV head) together are the M dimension of two
+// matrix products per 128-token tile, S = Q K^T and O += P V, so the shared
+// pages are read once per 256 rows instead of once per lane, and the products
+// are large enough for tcgen05. What the lanes have of their own goes through
+// the small-row path of the decode kernels. Both kinds of work run in one
+// launch, one thread block per item; every item leaves unnormalised FP32 partials
+// (O, row maximum, row sum) and a second, dependent launch joins each query
+// row's partials and rounds once to FP16.
+//
+// Shared item (one block per SM):
+//  * warp 8 walks the item's descriptors and fills a 4-stage ring with 128-token
+//    tiles of one KV head, K then V, [token][64 dims] with the 128-byte
+//    swizzle (TMA; an 8-token group is one swizzle atom, so pages of any size
+//    meet in a tile). A tile that is not full has the V rows of its invalid
+//    tokens zeroed in shared memory (0 * NaN would be NaN);
+//  * warp 9 issues the tcgen05.mma of both products: Q (TMEM, 128 rows) x K
+//    (shared memory) -> S (TMEM), P (TMEM) x V (shared memory, token rows =
+//    K dimension, i.e. MN-major) -> O (TMEM);
+//  * warps 0-3 and 4-7 are two softmax groups, one thread per query row. With
+//    two row tiles each group has a row tile of its own and both use every
+//    K/V tile; with one row tile they take the token tiles in turn and join at the
+//    end. While one group computes exponentials the tensor core works for
+//    the other.
+// P is handed to the FP16 product as hi + lo halves (p = hi + lo to 2^-21), so
+// that the weights keep FP32 precision as in the per-lane kernel; at 64 dims
+// the tensor core has the time, since the exponentials (16 per SM and clock)
+// bound a full tile: 1,024 clocks of them against 768 of products. The running
+// maximum is only raised, and O only rescaled, when a row's maximum grows by
+// more than 2^8 (P stays below 2^8 and within FP16; the quotient is exact in
+// either case).
+//
+// A lane's own pages: one warp per (lane, KV head, run of pages), 16-token
+// slices through a private cp.async ring, scores transposed (tokens x heads) on
+// m16n8k16 tiles: the products are at most 16 rows high, HBM bounds them.
+#include "../../../include/kk_kernels.h"
+#include "kernels_internal.h"
+#include "launch.cuh"
+
+#include <atomic>
+#include <cmath>
+
+namespace kk {
+
+__device__ unsigned int g_prefix_status;
+
+namespace {
+
+constexpr std::uint32_t kHeadDim = 64;
+constexpr std::uint32_t kRowBytes = kHeadDim * 2;
+constexpr std::uint32_t kSoftWarps = 8;
+constexpr std::uint32_t kProducerWarp = 8;
+constexpr std::uint32_t kIssuerWarp = 9;
+constexpr std::uint32_t kThreads = 384;               // three warpgroups; warps 10 and 11 only fill the third
+// A softmax thread holds a row of S (128 values); the third warpgroup gives up
+// registers for it. The block is launched with kLaunchRegs a thread, and the
+// three shares must fit into that.
+constexpr std::uint32_t kLaunchRegs = 168;
+constexpr std::uint32_t kSoftRegs = 216;
+constexpr std::uint32_t kFewRegs = 72;
+static_assert(2 * kSoftRegs + kFewRegs <= 3 * kLaunchRegs, "a share beyond the launch's registers never comes");
+constexpr std::uint32_t kStages = 4;
+constexpr std::uint32_t kTile = 128;                  // tokens per tile, and query rows per row tile
+constexpr std::uint32_t kSlots = kTile / 8;           // 8-token groups per tile
+constexpr std::uint32_t kHalfStage = kTile * kRowBytes;
+constexpr std::uint32_t kStageBytes = 2 * kHalfStage;
+constexpr std::uint64_t kAllValid = 0x8888888888888888ull;  // 8 tokens in each of 16 groups
+
+// TMEM columns.
+constexpr std::uint32_t kTmemCols = 512;
+constexpr std::uint32_t kColS = 0;      // two S tiles of 128 columns; P replaces S in place
+constexpr std::uint32_t kColO = 256;    // two O tiles of 64
+constexpr std::uint32_t kColQ = 384;    // two Q tiles of 32 (two FP16 per column)
+constexpr std::uint32_t kColPLo = 64;   // low halves of P, from the start of P
+
+// A lane's own pages.
+constexpr std::uint32_t kSlice = 16;                       // tokens per step
+constexpr std::uint32_t kSliceBytes = 2 * kSlice * kRowBytes;
+constexpr std::uint32_t kSliceRing = kStages * kStageBytes / kSoftWarps / kSliceBytes;  // 4
+static_assert(kSliceRing == 4, "the validity queue below holds four slices");
+
+constexpr float kRescale = 8.f;  // log2 growth of a row maximum that rescales O
+
+struct Args {
+    __half const* micro;
+    __half const* extent;
+    std::uint64_t micro_page;   // elements
+    std::uint64_t extent_page;
+    std::uint32_t micro_slots;
+    std::uint32_t extent_slots;
+    std::uint32_t micro_cap;
+    std::uint32_t layer;
+    std::uint32_t kv_heads;
+    std::uint32_t group;        // query heads per KV head
+    kk_prefix_plan plan;
+    kk_page_desc const* descs;
+    kk_attn_lane const* lanes;
+    kk_prefix_group const* groups;
+    kk_prefix_item const* items;
+    __half const* query;
+    __half* output;
+    std::uint64_t query_stride;
+    std::uint64_t output_stride;
+    float scale_log2;
+    float* part_o;              // [part_rows][64]
+    float2* part_ml;            // [part_rows] maximum (log2 units), sum
+};
+
+struct Maps {
+    CUtensorMap micro;       // boxes of a whole page
+    CUtensorMap micro8;      // boxes of 8 tokens
+    CUtensorMap extent;
+    CUtensorMap extent8;
+};
+
+struct Shared {  // behind the ring
+    std::uint64_t full[kStages];    // K and V landed
+    std::uint64_t fixed[kStages];   // V rows of invalid tokens are zero
+    std::uint64_t empty[kStages];   // the products are done with the stage
+    std::uint64_t s_full[2];        // S of softmax group w
+    std::uint64_t p_full[2];        // P of softmax group w
+    std::uint64_t q_full;
+    std::uint64_t o_full;
+    std::uint64_t valid[kStages];   // valid tokens of each 8-token group, 4 bits each
+    std::uint32_t tmem;
+    int abort;
+};
+
+constexpr std::size_t kSmemBytes = 1024 + kStages * kStageBytes + sizeof(Shared);
+
+__device__ __forceinline__ void report(unsigned int code) { atomicCAS(&g_prefix_status, kErrNone, code); }
+
+// Bounded wait that also ends when another warp gave up.
+__device__ __forceinline__ bool wait_or_abort(std::uint64_t* bar, std::uint32_t phase, int volatile* abort)
+{
+    if (mbar_poll(bar, phase)) {
+        return true;
+    }
+    std::uint64_t const t0 = global_ns();
+    for (std::uint32_t i = 0; i < kMaxWaitPolls; ++i) {
+        if (mbar_poll(bar, phase)) {
+            return true;
+        }
+        if (*abort) {
+            return false;
+        }
+        if (global_ns() - t0 > kWaitLimitNs) {
+            break;
+        }
+    }
+    *abort = 1;
+    report(kErrWaitTimeout);
+    return false;
+}
+
+__device__ __forceinline__ void tma_load_page(void* dst, CUtensorMap const* map, std::uint64_t* bar, int head,
+    int token, int block, int page)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+        ::"r"(smem_u32(dst)), "l"(reinterpret_cast<std::uint64_t>(map)), "r"(smem_u32(bar)),
+        "r"(0), "r"(head), "r"(token), "r"(block), "r"(page)
+        : "memory");
+}
+
+// D(tmem) (+)= A(tmem) * B(smem desc).
+__device__ __forceinline__ void mma_ts(std::uint32_t d, std::uint32_t a, std::uint64_t b, std::uint32_t idesc,
+    std::uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// 32 lanes x 32 columns; the caller waits.
+__device__ __forceinline__ void tmem_ld32(std::uint32_t addr, float* v)
+{
+    std::uint32_t* r = reinterpret_cast<std::uint32_t*>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32"
+        " {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21,"
+        " %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+}
+
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void tmem_st32(std::uint32_t addr, std::uint32_t const* r)
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0],"
+        " {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22,"
+        " %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+          "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+          "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_st16(std::uint32_t addr, std::uint32_t const (&r)[16])
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0],"
+        " {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+
+__device__ __forceinline__ float exp2_approx(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ std::uint32_t pack_half2(float lo, float hi)
+{
+    __half2 const h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<std::uint32_t const*>(&h);
+}
+
+// The leading 11 bits of p: what FP16 holds of it exactly (above its subnormals).
+__device__ __forceinline__ float leading(float p) { return __uint_as_float(__float_as_uint(p) & 0xffffe000u); }
+
+// ---- shared items -------------------------------------------------------------
+
+__device__ __forceinline__ void produce(Args const& a, Maps const& maps, kk_prefix_item const& item,
+    std::uint8_t* ring, Shared* sh)
+{
+    std::uint32_t const lane = threadIdx.x % 32u;
+    int volatile* abort = &sh->abort;
+    std::uint32_t win = item.desc_begin;
+    std::uint32_t w_slot = 0, w_word = 0, n_slot = 0, n_word = 0;
+    // 32 descriptors at a time, one per lane; the next ones are requested ahead.
+    auto fetch = [&](std::uint32_t at, std::uint32_t& slot, std::uint32_t& word) {
+        std::uint32_t const i = at + lane;
+        slot = word = 0;
+        if (i < item.desc_end) {
+            std::uint32_t const* d = reinterpret_cast<std::uint32_t const*>(a.descs + i);
+            slot = __ldg(d);
+            word = __ldg(d + 2);
+        }
+    };
+    fetch(win, w_slot, w_word);
+    fetch(win + 32u, n_slot, n_word);
+    std::uint32_t e = item.desc_begin;
+    std::uint32_t tile = 0;
+    int const block = static_cast<int>(a.layer * 2u);
+    int const head = static_cast<int>(item.kv_head);
+    bool ok = true;
+    for (; tile < item.token_tiles; ++tile) {
+        std::uint32_t const s = tile % kStages;
+        std::uint32_t const phase = (tile / kStages) & 1u;
+        ok = tile < kStages || wait_or_abort(&sh->empty[s], phase ^ 1u, abort);
+        if (!__all_sync(0xffffffffu, ok)) {
+            ok = false;
+            break;
+        }
+        std::uint8_t* const k_dst = ring + s * kStageBytes;
+        std::uint64_t valid = 0;
+        std::uint32_t n = 0;
+        for (; e < item.desc_end; ++e) {
+            if (e >= win + 32u) {
+                win += 32u;
+                w_slot = n_slot;
+                w_word = n_word;
+                fetch(win + 32u, n_slot, n_word);
+            }
+            std::uint32_t const slot = __shfl_sync(0xffffffffu, w_slot, e - win);
+            std::uint32_t const word = __shfl_sync(0xffffffffu, w_word, e - win);
+            std::uint32_t const tokens = word & 0xffffu;
+            std::uint32_t const kind = (word >> 16) & 0xffu;
+            std::uint32_t const cap = kind == 0 ? a.micro_cap : 64u;
+            if (kind > 1u || slot >= (kind == 0 ? a.micro_slots : a.extent_slots) || tokens > cap) {
+                if (lane == 0) {
+                    report(kErrBadDescriptor);
+                }
+                continue;
+            }
+            std::uint32_t const groups = (tokens + 7u) / 8u;
+            if (n + groups > kSlots) {
+                break;
+            }
+            bool const whole = groups * 8u == cap;
+            CUtensorMap const* map = kind == 0 ? (whole ? &maps.micro : &maps.micro8)
+                                               : (whole ? &maps.extent : &maps.extent8);
+            std::uint32_t const boxes = whole ? (groups != 0 ? 1u : 0u) : groups;
+            std::uint32_t const box = whole ? groups : 1u;  // groups per box
+            // Counted before the copies: the phase cannot end before the arrival below.
+            if (lane == 0 && boxes != 0) {
+                asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;"
+                             ::"r"(smem_u32(&sh->full[s])), "r"(2u * groups * 8u * kRowBytes)
+                             : "memory");
+                for (std::uint32_t b = 0; b < boxes; ++b) {
+                    std::uint8_t* dst = k_dst + (n + b * box) * 8u * kRowBytes;
+                    tma_load_page(dst, map, &sh->full[s], head, static_cast<int>(b * 8u), block,
+                        static_cast<int>(slot));
+                    tma_load_page(dst + kHalfStage, map, &sh->full[s], head, static_cast<int>(b * 8u), block + 1,
+                        static_cast<int>(slot));
+                }
+            }
+            for (std::uint32_t g = 0; g < groups; ++g) {
+                std::uint32_t const left = tokens - g * 8u;
+                valid |= std::uint64_t(left < 8u ? left : 8u) << (4u * (n + g));
+            }
+            n += groups;
+        }
+        if (lane == 0) {
+            sh->valid[s] = valid;
+            mbar_arrive(&sh->full[s]);  // releases valid; the phase ends when the bytes land
+        }
+        if (valid != kAllValid) {
+            ok = wait_or_abort(&sh->full[s], phase, abort);
+            if (!__all_sync(0xffffffffu, ok)) {
+                ok = false;
+                ++tile;
+                break;
+            }
+            std::uint8_t* const v = k_dst + kHalfStage;
+            for (std::uint32_t i = lane; i < kTile * 8u; i += 32u) {
+                std::uint32_t const t = i / 8u;
+                if (t % 8u >= ((valid >> (4u * (t / 8u))) & 15u)) {
+                    *reinterpret_cast<uint4*>(v + i * 16u) = make_uint4(0, 0, 0, 0);
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+        }
+        if (lane == 0) {
+            mbar_arrive(&sh->fixed[s]);
+        }
+    }
+    if (ok && lane == 0 && e < item.desc_end) {
+        report(kErrBadArgument);  // more pages than the item's tiles
+    }
+    if (!ok) {
+        // Nothing of this block may still be landing when it ends.
+        if (lane == 0) {
+            for (std::uint32_t j = tile > kStages ? tile - kStages : 0u; j < tile; ++j) {
+                mbar_wait(&sh->full[j % kStages], (j / kStages) & 1u, nullptr);
+            }
+        }
+        __syncwarp();
+    }
+}
+
+__device__ __forceinline__ void issue(kk_prefix_item const& item, std::uint8_t* ring, Shared* sh)
+{
+    int volatile* abort = &sh->abort;
+    std::uint32_t const tmem = sh->tmem;
+    std::uint32_t const n = item.token_tiles;
+    bool const pair = item.row_tiles == 2u;
+    constexpr std::uint32_t kIdescQK = umma_idesc_f16_f32(128, 128);
+    constexpr std::uint32_t kIdescPV = umma_idesc_f16_f32(128, 64) | (1u << 16);  // V is MN-major
+    auto landed = [&](std::uint32_t j) {
+        return wait_or_abort(&sh->full[j % kStages], (j / kStages) & 1u, abort);
+    };
+    auto qk = [&](std::uint32_t w, std::uint32_t j) {
+        std::uint64_t const k_desc = umma_desc_k_sw128(ring + (j % kStages) * kStageBytes);
+#pragma unroll
+        for (std::uint32_t k = 0; k < kHeadDim / 16u; ++k) {
+            mma_ts(tmem + kColS + w * kTile, tmem + kColQ + w * 32u + k * 8u, k_desc + k * 2u, kIdescQK, k != 0);
+        }
+        tc_commit(&sh->s_full[w]);
+    };
+    // P V of a group: FP16 high halves, then the low halves.
+    auto pv = [&](std::uint32_t w, std::uint32_t j, bool first) {
+        std::uint64_t const v_desc = umma_desc_k_sw128(ring + (j % kStages) * kStageBytes + kHalfStage);
+        std::uint32_t const p = tmem + kColS + w * kTile;
+        std::uint32_t const o = tmem + kColO + w * kHeadDim;
+#pragma unroll
+        for (std::uint32_t k = 0; k < kTile / 16u; ++k) {
+            std::uint64_t const b = v_desc + k * (16u * kRowBytes / 16u);
+            mma_ts(o, p + k * 8u, b, kIdescPV, !(first && k == 0));
+            mma_ts(o, p + kColPLo + k * 8u, b, kIdescPV, 1u);
+        }
+    };
+    auto weights = [&](std::uint32_t w, std::uint32_t k, std::uint32_t j) {  // the group's k-th P, on tile j
+        bool const ok = wait_or_abort(&sh->fixed[j % kStages], (j / kStages) & 1u, abort)
+            && wait_or_abort(&sh->p_full[w], k & 1u, abort);
+        tc_fence_after();
+        return ok;
+    };
+    bool ok = wait_or_abort(&sh->q_full, 0, abort) && landed(0);
+    tc_fence_after();
+    if (ok) {
+        qk(0, 0);
+        if (pair) {
+            qk(1, 0);
+        } else if (n > 1u) {
+            ok = landed(1);
+            if (ok) {
+                qk(1, 1);
+            }
+        }
+    }
+    // The product that overwrites S of a group is issued behind the one that
+    // reads P from the same columns; the tensor core runs them in that order.
+    for (std::uint32_t j = 0; ok && j < n; ++j) {
+        if (pair) {
+            for (std::uint32_t w = 0; w < 2u && ok; ++w) {
+                ok = weights(w, j, j);
+                if (!ok) {
+                    break;
+                }
+                pv(w, j, j == 0);
+                if (w == 1u) {
+                    tc_commit(&sh->empty[j % kStages]);
+                }
+                if (j + 1u < n) {
+                    ok = landed(j + 1u);
+                    if (ok) {
+                        qk(w, j + 1u);
+                    }
+                }
+            }
+        } else {
+            std::uint32_t const w = j & 1u;
+            ok = weights(w, j >> 1, j);
+            if (!ok) {
+                break;
+            }
+            pv(w, j, j < 2u);
+            tc_commit(&sh->empty[j % kStages]);
+            if (j + 2u < n) {
+                ok = landed(j + 2u);
+                if (ok) {
+                    qk(w, j + 2u);
+                }
+            }
+        }
+    }
+    tc_commit(&sh->o_full);
+    if (!ok) {
+        mbar_wait(&sh->o_full, 0, nullptr);  // no product outlives the TMEM
+    }
+}
+
+// One thread per query row: warp % 4 selects the TMEM lanes, warp / 4 the group.
+__device__ __forceinline__ void soften(Args const& a, kk_prefix_item const& item, kk_prefix_group const& g,
+    std::uint8_t* ring, Shared* sh)
+{
+    int volatile* abort = &sh->abort;
+    std::uint32_t const warp = threadIdx.x / 32u;
+    std::uint32_t const lane = threadIdx.x % 32u;
+    std::uint32_t const w = warp / 4u;
+    bool const pair = item.row_tiles == 2u;
+    std::uint32_t const r = (warp % 4u) * 32u + lane;
+    std::uint32_t const tile_row = (item.row_tile + (pair ? w : 0u)) * kTile;
+    std::uint32_t const rows = g.lane_count * a.group;
+    bool const mine = tile_row + r < rows;
+    bool const any = tile_row + (warp % 4u) * 32u < rows;  // some row of this warp exists
+    std::uint32_t const tmem = sh->tmem + ((warp % 4u) * 32u << 16);
+    std::uint32_t const s_col = tmem + kColS + w * kTile;
+    std::uint32_t const o_col = tmem + kColO + w * kHeadDim;
+
+    {
+        std::uint32_t q[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            q[i] = 0;
+        }
+        if (mine) {
+            std::uint32_t const row = tile_row + r;
+            std::uint32_t const query_row = a.lanes[g.lane_begin + row / a.group].query_row;
+            uint4 const* src = reinterpret_cast<uint4 const*>(a.query + query_row * a.query_stride
+                + (item.kv_head * a.group + row % a.group) * kHeadDim);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                uint4 const x = src[i];
+                q[4 * i] = x.x;
+                q[4 * i + 1] = x.y;
+                q[4 * i + 2] = x.z;
+                q[4 * i + 3] = x.w;
+            }
+        }
+        tmem_st32(tmem + kColQ + w * 32u, q);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+            mbar_arrive(&sh->q_full);
+        }
+    }
+
+    float m = -INFINITY;  // reference maximum of the row, log2 units
+    float l = 0.f;
+    std::uint32_t k = 0;
+    bool ok = true;
+    for (std::uint32_t j = pair ? 0u : w; j < item.token_tiles; j += pair ? 1u : 2u, ++k) {
+        std::uint32_t const s = j % kStages;
+        ok = wait_or_abort(&sh->full[s], (j / kStages) & 1u, abort)
+            && wait_or_abort(&sh->s_full[w], k & 1u, abort);
+        if (!__all_sync(0xffffffffu, ok)) {
+            ok = false;
+            break;
+        }
+        tc_fence_after();
+        if (any) {
+            float x[kTile];
+#pragma unroll
+            for (std::uint32_t c = 0; c < 4u; ++c) {
+                tmem_ld32(s_col + c * 32u, x + c * 32u);
+            }
+            std::uint64_t const valid = sh->valid[s];
+            tmem_wait_ld();
+            if (valid != kAllValid) {
+#pragma unroll
+                for (std::uint32_t i = 0; i < kTile; ++i) {
+                    x[i] = (i % 8u) < (static_cast<std::uint32_t>(valid >> (4u * (i / 8u))) & 15u) ? x[i] : -INFINITY;
+                }
+            }
+            float top[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+            for (std::uint32_t i = 4; i < kTile; ++i) {
+                top[i % 4u] = fmaxf(top[i % 4u], x[i]);
+            }
+            float const mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
+            bool const grow = mt > m + kRescale || m == -INFINITY;
+            if (__any_sync(0xffffffffu, grow)) {
+                float const m_new = grow ? mt : m;
+                float const alpha = m == -INFINITY || !grow ? 1.f : exp2_approx(m - m_new);
+                m = m_new;
+                l *= alpha;
+                if (k != 0) {
+                    // S of this tile was issued behind the previous P V, so O is at rest.
+#pragma unroll
+                    for (std::uint32_t c = 0; c < 2u; ++c) {
+                        float o[32];
+                        tmem_ld32(o_col + c * 32u, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            o[i] *= alpha;
+                        }
+                        tmem_st32(o_col + c * 32u, reinterpret_cast<std::uint32_t const*>(o));
+                    }
+                }
+            }
+            float const m_use = m == -INFINITY ? 0.f : m;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (std::uint32_t c = 0; c < 4u; ++c) {
+                std::uint32_t hi[16], lo[16];
+#pragma unroll
+                for (std::uint32_t i = 0; i < 16u; ++i) {
+                    float const p0 = exp2_approx(fmaf(x[c * 32u + 2u * i], a.scale_log2, -m_use));
+                    float const p1 = exp2_approx(fmaf(x[c * 32u + 2u * i + 1u], a.scale_log2, -m_use));
+                    sum[(2u * i) % 4u] += p0;
+                    sum[(2u * i + 1u) % 4u] += p1;
+                    float const h0 = leading(p0), h1 = leading(p1);
+                    hi[i] = pack_half2(h0, h1);
+                    lo[i] = pack_half2(p0 - h0, p1 - h1);
+                }
+                tmem_st16(s_col + c * 16u, hi);
+                tmem_st16(s_col + kColPLo + c * 16u, lo);
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tmem_wait_st();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+            mbar_arrive(&sh->p_full[w]);
+        }
+    }
+    ok = ok && wait_or_abort(&sh->o_full, 0, abort);
+    ok = __all_sync(0xffffffffu, ok);
+    tc_fence_after();
+    float o[kHeadDim];
+    if (ok && any && k != 0) {
+        tmem_ld32(o_col, o);
+        tmem_ld32(o_col + 32u, o + 32);
+        tmem_wait_ld();
+    } else {
+#pragma unroll
+        for (std::uint32_t i = 0; i < kHeadDim; ++i) {
+            o[i] = 0.f;
+        }
+    }
+    // One row tile: the second group's half of the tokens joins the first's
+    // through the ring, which nothing uses any more.
+    constexpr std::uint32_t kStride = kHeadDim + 3;  // odd: rows fall into different banks
+    float* const join = reinterpret_cast<float*>(ring) + r * kStride;
+    if (!pair && w == 1u && ok) {
+#pragma unroll
+        for (std::uint32_t i = 0; i < kHeadDim; ++i) {
+            join[i] = o[i];
+        }
+        join[kHeadDim] = m;
+        join[kHeadDim + 1] = l;
+    }
+    asm volatile("bar.sync 1, 256;" ::: "memory");  // the 8 softmax warps, all of which come here
+    if (!pair && (w == 1u || !ok)) {
+        return;
+    }
+    if (!pair) {
+        float const m1 = join[kHeadDim];
+        float const top = fmaxf(m, m1);
+        float const use = top == -INFINITY ? 0.f : top;
+        float const f0 = exp2_approx(m - use), f1 = exp2_approx(m1 - use);
+        m = top;
+        l = l * f0 + join[kHeadDim + 1] * f1;
+#pragma unroll
+        for (std::uint32_t i = 0; i < kHeadDim; ++i) {
+            o[i] = o[i] * f0 + join[i] * f1;
+        }
+    }
+    if (mine && ok) {
+        std::uint64_t const row = g.part_row
+            + (std::uint64_t(item.kv_head * g.part_count + item.part) * g.row_tiles) * kTile + tile_row + r;
+        float4* dst = reinterpret_cast<float4*>(a.part_o + row * kHeadDim);
+#pragma unroll
+        for (std::uint32_t i = 0; i < kHeadDim / 4u; ++i) {
+            dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        }
+        a.part_ml[row] = make_float2(m, l);
+    }
+}
+
+// ---- a lane's own pages -------------------------------------------------------
+
+__device__ __forceinline__ void cp_async16(std::uint32_t dst, void const* src)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+__device__ __forceinline__ void ldsm_x4(std::uint32_t addr, std::uint32_t (&r)[4])
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
+__device__ __forceinline__ void ldsm_x4_t(std::uint32_t addr, std::uint32_t (&r)[4])
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
+__device__ __forceinline__ void mma16816(float (&d)[4], std::uint32_t a0, std::uint32_t a1, std::uint32_t a2,
+    std::uint32_t a3, std::uint32_t b0, std::uint32_t b1)
+{
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+        "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ std::uint32_t transpose8x8(std::uint32_t x)
+{
+    std::uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+// One (lane, KV head, run of pages) by one warp. NT: tiles of 8 query heads.
+template <int NT>
+__device__ __forceinline__ void own_task(Args const& a, kk_prefix_item const& item, std::uint8_t* warp_ring)
+{
+    std::uint32_t const lane = threadIdx.x % 32u;
+    std::uint32_t const g = lane >> 2;
+    std::uint32_t const c4 = lane & 3u;
+    std::uint32_t const mi = lane >> 3;
+    std::uint32_t const r8 = lane & 7u;
+    std::uint32_t const G = a.group;
+    kk_attn_lane const ln = a.lanes[item.owner];
+    std::uint64_t const row0 = std::uint64_t(ln.item_offset) + std::uint64_t(item.part) * a.plan.q_heads
+        + item.kv_head * G;
+    if (item.part >= ln.item_count || row0 + G > a.plan.part_rows) {
+        if (lane == 0) {
+            report(kErrBadArgument);
+        }
+        return;
+    }
+    // Queries as B fragments of S^T = K Q^T; heads past the group are zero.
+    std::uint32_t qf[NT][4][2];
+    {
+        __half const* q = a.query + ln.query_row * a.query_stride + item.kv_head * G * kHeadDim;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            std::uint32_t const h = nt * 8u + g;
+#pragma unroll
+            for (int k16 = 0; k16 < 4; ++k16) {
+#pragma unroll
+                for (int hi = 0; hi < 2; ++hi) {
+                    qf[nt][k16][hi] = h < G ? *reinterpret_cast<std::uint32_t const*>(
+                        q + h * kHeadDim + k16 * 16 + hi * 8 + c4 * 2u) : 0u;
+                }
+            }
+        }
+    }
+    // Cursor over 8-token groups.
+    std::uint32_t const row = a.kv_heads * kHeadDim;  // elements per token
+    std::uint32_t win = item.desc_begin;
+    std::uint32_t w_slot = 0, w_word = 0;
+    auto fetch = [&]() {
+        std::uint32_t const i = win + lane;
+        w_slot = w_word = 0;
+        if (i < item.desc_end) {
+            std::uint32_t const* d = reinterpret_cast<std::uint32_t const*>(a.descs + i);
+            w_slot = __ldg(d);
+            w_word = __ldg(d + 2);
+        }
+    };
+    fetch();
+    std::uint32_t e = item.desc_begin, token = 0;
+    __half const* src = nullptr;   // K of the next group's first token; V follows after v_off elements
+    std::uint32_t v_off = 0;
+    // Moves to the next group; its valid tokens, 0 at the end.
+    auto next_group = [&](__half const*& at, std::uint32_t& off) -> std::uint32_t {
+        for (; e < item.desc_end; ++e, token = 0) {
+            if (e >= win + 32u) {
+                win += 32u;
+                fetch();
+            }
+            std::uint32_t const slot = __shfl_sync(0xffffffffu, w_slot, e - win);
+            std::uint32_t const word = __shfl_sync(0xffffffffu, w_word, e - win);
+            std::uint32_t const tokens = word & 0xffffu;
+            std::uint32_t const kind = (word >> 16) & 0xffu;
+            std::uint32_t const cap = kind == 0 ? a.micro_cap : 64u;
+            if (kind > 1u || slot >= (kind == 0 ? a.micro_slots : a.extent_slots) || tokens > cap) {
+                if (lane == 0) {
+                    report(kErrBadDescriptor);
+                }
+                continue;
+            }
+            if (token >= tokens) {
+                continue;
+            }
+            __half const* page = kind == 0 ? a.micro + slot * a.micro_page : a.extent + slot * a.extent_page;
+            v_off = cap * row;
+            src = page + std::uint64_t(a.layer) * 2u * v_off + token * row + item.kv_head * kHeadDim;
+            std::uint32_t const left = tokens - token;
+            token += 8u;
+            at = src;
+            off = v_off;
+            return left < 8u ? left : 8u;
+        }
+        return 0u;
+    };
+    std::uint32_t const ring = smem_u32(warp_ring);
+    std::uint32_t queue = 0;  // valid tokens of the slices in flight: 8 bits each, newest highest
+    std::uint32_t head_slice = 0;  // slices requested
+    auto request = [&]() {  // one slice (or nothing) into the ring, always one commit group
+        __half const* at0 = nullptr;
+        __half const* at1 = nullptr;
+        std::uint32_t off0 = 0, off1 = 0;
+        std::uint32_t const v0 = next_group(at0, off0);
+        std::uint32_t const v1 = v0 != 0 ? next_group(at1, off1) : 0u;
+        std::uint32_t const dst = ring + (head_slice % kSliceRing) * kSliceBytes;
+        std::uint32_t const ch = lane & 7u;
+#pragma unroll
+        for (std::uint32_t i = 0; i < 4u; ++i) {
+            std::uint32_t const t = (lane >> 3) + 4u * i;   // token of the slice
+            std::uint32_t const in_group = t & 7u;
+            if ((i < 2u ? v0 : v1) > in_group) {
+                __half const* p = (i < 2u ? at0 : at1) + in_group * row + ch * 8u;
+                std::uint32_t const o = t * kRowBytes + ((ch ^ in_group) << 4);
+                cp_async16(dst + o, p);
+                cp_async16(dst + kSlice * kRowBytes + o, p + (i < 2u ? off0 : off1));
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        queue = (queue >> 8) | ((v0 | (v1 << 4)) << 24);
+        ++head_slice;
+    };
+    float mrow[NT][2], lrow[NT][2], o[NT][4][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        mrow[nt][0] = mrow[nt][1] = -INFINITY;
+        lrow[nt][0] = lrow[nt][1] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
+        }
+    }
+    request();
+    request();
+    request();
+    for (std::uint32_t slice = 0;; ++slice) {
+        // The slice in turn is the third newest; it is the oldest with tokens left.
+        std::uint32_t const pairv = (queue >> 8) & 0xffu;
+        if (pairv == 0) {
+            break;
+        }
+        request();
+        asm volatile("cp.async.wait_group 3;" ::: "memory");
+        __syncwarp();
+        std::uint32_t const v0 = pairv & 15u, v1 = pairv >> 4;
+        std::uint32_t const kbase = ring + (slice % kSliceRing) * kSliceBytes;
+        std::uint32_t const vbase = kbase + kSlice * kRowBytes;
+        float st[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            st[nt][0] = st[nt][1] = st[nt][2] = st[nt][3] = 0.f;
+        }
+#pragma unroll
+        for (std::uint32_t k16 = 0; k16 < 4; ++k16) {
+            std::uint32_t const tr = (mi & 1u) * 8u + r8;
+            std::uint32_t const ch = 2u * k16 + (mi >> 1);
+            std::uint32_t ka[4];
+            ldsm_x4(kbase + tr * kRowBytes + ((ch ^ r8) << 4), ka);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                mma16816(st[nt], ka[0], ka[1], ka[2], ka[3], qf[nt][k16][0], qf[nt][k16][1]);
+            }
+        }
+        bool const tg = g < v0, tg8 = g < v1;
+        // V of masked tokens is zeroed: bytes past the valid tokens are never trusted.
+        std::uint32_t const mask0 = (2 * c4 < v0 ? 0x0000ffffu : 0u) | (2 * c4 + 1 < v0 ? 0xffff0000u : 0u);
+        std::uint32_t const mask1 = (2 * c4 < v1 ? 0x0000ffffu : 0u) | (2 * c4 + 1 < v1 ? 0xffff0000u : 0u);
+        std::uint32_t pb[NT][2], pl[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float p[4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float const xa = tg ? st[nt][h] * a.scale_log2 : -INFINITY;
+                float const xb = tg8 ? st[nt][2 + h] * a.scale_log2 : -INFINITY;
+                float mx = fmaxf(xa, xb);
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                float const m_new = fmaxf(mrow[nt][h], mx);
+                float const m_use = m_new == -INFINITY ? 0.f : m_new;
+                float const alpha = exp2_approx(mrow[nt][h] - m_use);
+                p[h] = exp2_approx(xa - m_use);
+                p[2 + h] = exp2_approx(xb - m_use);
+                lrow[nt][h] = lrow[nt][h] * alpha + p[h] + p[2 + h];
+                mrow[nt][h] = m_new;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    o[nt][j][h] *= alpha;
+                    o[nt][j][2 + h] *= alpha;
+                }
+            }
+            float hp[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                hp[i] = leading(p[i]);
+            }
+            pb[nt][0] = transpose8x8(pack_half2(hp[0], hp[1]));
+            pb[nt][1] = transpose8x8(pack_half2(hp[2], hp[3]));
+            pl[nt][0] = transpose8x8(pack_half2(p[0] - hp[0], p[1] - hp[1]));
+            pl[nt][1] = transpose8x8(pack_half2(p[2] - hp[2], p[3] - hp[3]));
+        }
+#pragma unroll
+        for (std::uint32_t j = 0; j < 4; ++j) {
+            std::uint32_t const tr = (mi >> 1) * 8u + r8;
+            std::uint32_t const ch = 2u * j + (mi & 1u);
+            std::uint32_t va[4];
+            ldsm_x4_t(vbase + tr * kRowBytes + ((ch ^ r8) << 4), va);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                mma16816(o[nt][j], va[0] & mask0, va[1] & mask0, va[2] & mask1, va[3] & mask1, pb[nt][0], pb[nt][1]);
+                mma16816(o[nt][j], va[0] & mask0, va[1] & mask0, va[2] & mask1, va[3] & mask1, pl[nt][0], pl[nt][1]);
+            }
+        }
+        __syncwarp();  // the slice's slot is requested again in the next step
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float l = lrow[nt][h];
+            l += __shfl_xor_sync(0xffffffffu, l, 4);
+            l += __shfl_xor_sync(0xffffffffu, l, 8);
+            l += __shfl_xor_sync(0xffffffffu, l, 16);
+            std::uint32_t const qh = nt * 8u + 2u * c4 + h;
+            if (qh < G) {
+                float* dst = a.part_o + (row0 + qh) * kHeadDim;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    dst[16 * j + g] = o[nt][j][h];
+                    dst[16 * j + 8 + g] = o[nt][j][2 + h];
+                }
+                if (g == 0) {
+                    a.part_ml[row0 + qh] = make_float2(mrow[nt][h], l);
+                }
+            }
+        }
+    }
+    __syncwarp();
+}
+
+template <int NT>
+__global__ void __launch_bounds__(kThreads, 1) prefix_attention_kernel(const __grid_constant__ Maps maps,
+    const __grid_constant__ Args a)
+{
+    extern __shared__ std::uint8_t smem_raw[];
+    std::uint32_t const pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;  // swizzle atoms are 1 KB
+    std::uint8_t* const ring = smem_raw + pad;
+    Shared* const sh = reinterpret_cast<Shared*>(ring + kStages * kStageBytes);
+    std::uint32_t const warp = threadIdx.x / 32u;
+    pdl_launch_dependents();
+    if (blockIdx.x >= a.plan.num_shared) {
+        pdl_wait();
+        if (warp >= kSoftWarps) {
+            return;
+        }
+        std::uint32_t const own = a.plan.num_items - a.plan.num_shared;
+        std::uint32_t const first = (blockIdx.x - a.plan.num_shared) * a.plan.tasks_per_cta;
+        std::uint32_t const left = own - first;
+        std::uint32_t const count = left < a.plan.tasks_per_cta ? left : a.plan.tasks_per_cta;
+        for (std::uint32_t t = warp; t < count; t += kSoftWarps) {
+            kk_prefix_item const item = a.items[a.plan.num_shared + first + t];
+            if (item.row_tiles != 0 || item.owner >= a.plan.num_lanes || item.kv_head >= a.kv_heads
+                || item.desc_begin > item.desc_end || item.desc_end > a.plan.num_descs) {
+                if (threadIdx.x % 32u == 0) {
+                    report(kErrBadArgument);
+                }
+                continue;
+            }
+            own_task<NT>(a, item, ring + warp * kSliceRing * kSliceBytes);
+        }
+        return;
+    }
+    if (threadIdx.x == 0) {
+        for (std::uint32_t s = 0; s < kStages; ++s) {
+            mbar_init(&sh->full[s], 1);
+            mbar_init(&sh->fixed[s], 1);
+            mbar_init(&sh->empty[s], 1);
+        }
+        for (int w = 0; w < 2; ++w) {
+            mbar_init(&sh->s_full[w], 1);
+            mbar_init(&sh->p_full[w], 4);
+        }
+        mbar_init(&sh->q_full, kSoftWarps);
+        mbar_init(&sh->o_full, 1);
+        sh->abort = 0;
+        fence_barrier_init();
+    }
+    pdl_wait();
+    kk_prefix_item const item = a.items[blockIdx.x];
+    kk_prefix_group g{};
+    bool fits = item.owner < a.plan.num_groups;
+    if (fits) {
+        g = a.groups[item.owner];
+        fits = (item.row_tiles == 1u || item.row_tiles == 2u) && item.kv_head < a.kv_heads
+            && item.desc_begin <= item.desc_end && item.desc_end <= a.plan.num_descs && item.token_tiles != 0
+            && item.row_tile + item.row_tiles <= g.row_tiles && item.part < g.part_count
+            && g.lane_begin <= a.plan.num_lanes && g.lane_count <= a.plan.num_lanes - g.lane_begin
+            && std::uint64_t(g.part_row) + std::uint64_t(a.kv_heads) * g.part_count * g.row_tiles * kTile
+                <= a.plan.part_rows;
+    }
+    if (!fits) {  // the same for every thread
+        if (threadIdx.x == 0) {
+            report(kErrBadArgument);
+        }
+        return;
+    }
+    if (warp == kIssuerWarp) {
+        tmem_alloc(&sh->tmem, kTmemCols);
+        tmem_relinquish();
+        tc_fence_before();
+    }
+    __syncthreads();
+    tc_fence_after();
+    if (warp < kSoftWarps) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
+        soften(a, item, g, ring, sh);
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
+        if (warp == kProducerWarp) {
+            produce(a, maps, item, ring, sh);
+        } else if (warp == kIssuerWarp) {
+            if (threadIdx.x % 32u == 0) {
+                issue(item, ring, sh);
+            }
+            __syncwarp();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kIssuerWarp) {
+        tc_fence_after();
+        tmem_dealloc(sh->tmem, kTmemCols);
+    }
+}
+
+// ---- joining the partials -----------------------------------------------------
+
+constexpr std::uint32_t kJoinThreads = 256;
+constexpr std::uint32_t kJoinBatch = 8;  // partials requested at once
+
+// 16 threads per query row, 4 dims each: out = sum_i 2^(m_i - m) O_i / sum_i
+// 2^(m_i - m) l_i over the row's partials, in their order.
+__global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(const __grid_constant__ Args a)
+{
+    pdl_launch_dependents();
+    pdl_wait();
+    std::uint32_t const t = blockIdx.x * kJoinThreads + threadIdx.x;
+    std::uint32_t const q_heads = a.plan.q_heads;
+    std::uint32_t const lane = t / 16u / q_heads;
+    if (lane >= a.plan.num_lanes) {
+        return;
+    }
+    std::uint32_t const qh = t / 16u % q_heads;
+    std::uint32_t const d0 = t % 16u * 4u;
+    kk_attn_lane const ln = a.lanes[lane];
+    std::uint64_t base = 0, step = 0;
+    std::uint32_t shared = 0;
+    if (ln.reserved - 1u < a.plan.num_groups) {
+        kk_prefix_group const g = a.groups[ln.reserved - 1u];
+        step = std::uint64_t(g.row_tiles) * kTile;
+        shared = g.part_count;
+        base = g.part_row + std::uint64_t(qh / a.group) * shared * step + (lane - g.lane_begin) * a.group + qh % a.group;
+    }
+    std::uint32_t const count = shared + ln.item_count;
+    std::uint64_t const own = std::uint64_t(ln.item_offset) + qh;
+    bool const fits = (shared == 0 || base + (shared - 1u) * step < a.plan.part_rows)
+        && (ln.item_count == 0 || own + std::uint64_t(ln.item_count - 1u) * q_heads < a.plan.part_rows);
+    if (!fits) {
+        report(kErrBadArgument);
+        return;
+    }
+    float m = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (std::uint32_t i0 = 0; i0 < count; i0 += kJoinBatch) {
+        float2 ml[kJoinBatch];
+        float4 o[kJoinBatch];
+#pragma unroll
+        for (std::uint32_t k = 0; k < kJoinBatch; ++k) {
+            std::uint32_t const i = i0 + k;
+            ml[k] = make_float2(-INFINITY, 0.f);
+            o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (i < count) {
+                std::uint64_t const row = i < shared ? base + i * step : own + std::uint64_t(i - shared) * q_heads;
+                ml[k] = __ldcg(a.part_ml + row);
+                o[k] = __ldcg(reinterpret_cast<float4 const*>(a.part_o + row * kHeadDim + d0));
+            }
+        }
+#pragma unroll
+        for (std::uint32_t k = 0; k < kJoinBatch; ++k) {
+            float const m_new = fmaxf(m, ml[k].x);
+            float const use = m_new == -INFINITY ? 0.f : m_new;
+            float const f = exp2_approx(m - use);
+            float const fk = exp2_approx(ml[k].x - use);
+            m = m_new;
+            l = l * f + ml[k].y * fk;
+            acc.x = acc.x * f + o[k].x * fk;
+            acc.y = acc.y * f + o[k].y * fk;
+            acc.z = acc.z * f + o[k].z * fk;
+            acc.w = acc.w * f + o[k].w * fk;
+        }
+    }
+    float const inv = l == 0.f ? 0.f : 1.f / l;  // no tokens at all: zeros
+    uint2 out;
+    out.x = pack_half2(acc.x * inv, acc.y * inv);
+    out.y = pack_half2(acc.z * inv, acc.w * inv);
+    *reinterpret_cast<uint2*>(a.output + ln.query_row * a.output_stride + qh * kHeadDim + d0) = out;
+}
+
+// Kernel attributes are set once per device.
+cudaError_t allowSharedMemory()
+{
+    static std::atomic<std::uint64_t> done{0};
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess || (device < 64 && (done.load(std::memory_order_acquire) >> device & 1u) != 0)) {
+        return e;
+    }
+    void const* const kernels[] = {reinterpret_cast<void const*>(prefix_attention_kernel<1>),
+        reinterpret_cast<void const*>(prefix_attention_kernel<2>)};
+    for (void const* kernel : kernels) {
+        // The register shares wait for ever in a build that launches with fewer.
+        cudaFuncAttributes attr{};
+        e = e == cudaSuccess ? cudaFuncGetAttributes(&attr, kernel) : e;
+        if (e == cudaSuccess && attr.numRegs < static_cast<int>(kLaunchRegs)) {
+            e = cudaErrorInvalidKernelImage;
+        }
+        if (e == cudaSuccess) {
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemBytes));
+        }
+    }
+    if (e == cudaSuccess && device < 64) {
+        done.fetch_or(std::uint64_t(1) << device, std::memory_order_release);
+    }
+    return e;
+}
+
+// ---- planning -------------------------------------------------------------------
+
+// Measured costs of a thread block's work, in nanoseconds, that decide how
+// many splits the prefixes get against the lanes' own pages.
+constexpr double kTilePairNs = 1200.;   // a 128-token tile for two row tiles
+constexpr double kTileSingleNs = 620.;  // for one
+constexpr double kOwnTokenNs = 5.7;     // a token of one KV head: 256 bytes at an SM's share of HBM
+constexpr std::uint32_t kOwnMinTokens = 64;
+
+std::uint32_t groupsOf(kk_page_desc const& d) { return d.valid_tokens > 64u ? 0u : (d.valid_tokens + 7u) / 8u; }
+
+// 128-token tiles of a run of descriptors, filled as the kernel does; calls
+// cut(tiles closed so far, first descriptor of the next tile) at every tile's end
+// but the last.
+template <typename Cut>
+std::uint32_t walkTiles(kk_page_desc const* descs, std::uint32_t begin, std::uint32_t end, Cut&& cut)
+{
+    std::uint32_t closed = 0, n = 0;
+    for (std::uint32_t e = begin; e < end; ++e) {
+        std::uint32_t const g = groupsOf(descs[e]);
+        if (n + g > kSlots) {
+            cut(++closed, e);
+            n = 0;
+        }
+        n += g;
+    }
+    return closed + (n != 0 ? 1u : 0u);
+}
+
+bool headsServed(std::uint32_t q_heads, std::uint32_t kv_heads)
+{
+    return kv_heads != 0 && q_heads != 0 && q_heads % kv_heads == 0 && q_heads / kv_heads <= 16u && q_heads <= 4096u;
+}
+
+} // namespace
+
+int prefixStatus(cudaStream_t stream) { return readStatus(&g_prefix_status, stream); }
+
+} // namespace kk
+
+extern "C" {
+
+uint32_t kk_prefix_groups(const kk_page_desc* descs, kk_attn_lane* lanes, uint32_t num_lanes, uint32_t min_lanes,
+    uint32_t min_tokens, kk_prefix_group* groups, uint32_t max_groups)
+{
+    if (descs == nullptr || lanes == nullptr || groups == nullptr) {
+        return 0;
+    }
+    auto same = [](kk_page_desc const& x, kk_page_desc const& y) {
+        return x.slot == y.slot && x.kind == y.kind && x.valid_tokens == y.valid_tokens;
+    };
+    min_lanes = min_lanes < 2u ? 2u : min_lanes;
+    std::uint32_t found = 0;
+    for (std::uint32_t b = 0; found < max_groups && num_lanes - b >= min_lanes;) {
+        kk_page_desc const* const first = descs + lanes[b].desc_offset;
+        auto common = [&](kk_attn_lane const& other, std::uint32_t most) {
+            std::uint32_t n = 0;
+            while (n < most && n < other.desc_count && same(first[n], descs[other.desc_offset + n])) {
+                ++n;
+            }
+            return n;
+        };
+        std::uint32_t const pages = common(lanes[b + 1], lanes[b].desc_count);
+        std::uint64_t tokens = 0;
+        for (std::uint32_t n = 0; n < pages; ++n) {
+            tokens += first[n].valid_tokens;
+        }
+        std::uint32_t end = b + 2u;
+        if (pages != 0 && tokens >= min_tokens) {
+            while (end < num_lanes && common(lanes[end], pages) == pages) {
+                ++end;
+            }
+        }
+        if (pages == 0 || tokens < min_tokens || end - b < min_lanes) {
+            ++b;
+            continue;
+        }
+        std::uint32_t const count = static_cast<std::uint32_t>(tokens);
+        groups[found++] = kk_prefix_group{lanes[b].desc_offset, pages, count, b, end - b, 0, 0, 0};
+        for (; b < end; ++b) {
+            lanes[b].desc_offset += pages;
+            lanes[b].desc_count -= pages;
+            lanes[b].token_count -= lanes[b].token_count < count ? lanes[b].token_count : count;
+        }
+    }
+    return found;
+}
+
+int kk_prefix_attention_plan(const kk_page_desc* descs, uint32_t num_descs, kk_attn_lane* lanes, uint32_t num_lanes,
+    kk_prefix_group* groups, uint32_t num_groups, uint32_t q_heads, uint32_t kv_heads, uint32_t num_sms,
+    kk_prefix_item* items, uint32_t max_items, kk_prefix_plan* plan)
+{
+    using namespace kk;
+    if (plan == nullptr || !headsServed(q_heads, kv_heads) || num_sms == 0 || (num_descs != 0 && descs == nullptr)
+        || (num_lanes != 0 && lanes == nullptr) || (num_groups != 0 && groups == nullptr)
+        || (max_items != 0 && items == nullptr)) {
+        return KK_EINVAL;
+    }
+    *plan = kk_prefix_plan{0, 0, kSoftWarps, num_lanes, num_groups, num_descs, q_heads, kv_heads, 0};
+    std::uint32_t const ratio = q_heads / kv_heads;
+    auto outside = [&](std::uint32_t offset, std::uint32_t count) {
+        return offset > num_descs || count > num_descs - offset;
+    };
+    std::uint64_t own_tokens = 0;
+    for (std::uint32_t b = 0; b < num_lanes; ++b) {
+        kk_attn_lane& ln = lanes[b];
+        if (outside(ln.desc_offset, ln.desc_count)) {
+            return KK_EINVAL;
+        }
+        ln.item_offset = ln.item_count = ln.reserved = 0;
+        for (std::uint32_t e = ln.desc_offset; e < ln.desc_offset + ln.desc_count; ++e) {
+            own_tokens += 8u * groupsOf(descs[e]);
+        }
+    }
+    // A prefix's tiles and what one KV head's rows cost on it.
+    auto tilesOf = [&](kk_prefix_group const& g) {
+        return walkTiles(descs, g.desc_offset, g.desc_offset + g.desc_count, [](std::uint32_t, std::uint32_t) {});
+    };
+    auto unitNs = [](kk_prefix_group const& g) { return g.row_tiles > 1u ? kTilePairNs : kTileSingleNs; };
+    double total = static_cast<double>(own_tokens) * kv_heads * kOwnTokenNs;
+    for (std::uint32_t i = 0; i < num_groups; ++i) {
+        kk_prefix_group& g = groups[i];
+        if (outside(g.desc_offset, g.desc_count) || g.lane_begin > num_lanes
+            || g.lane_count > num_lanes - g.lane_begin) {
+            return KK_EINVAL;
+        }
+        std::uint64_t const row_tiles = (std::uint64_t(g.lane_count) * ratio + kTile - 1u) / kTile;
+        if (row_tiles > 65535u) {
+            return KK_EINVAL;
+        }
+        g.row_tiles = static_cast<std::uint32_t>(row_tiles);
+        for (std::uint32_t b = g.lane_begin; b < g.lane_begin + g.lane_count; ++b) {
+            if (lanes[b].reserved != 0) {
+                return KK_EINVAL;
+            }
+            lanes[b].reserved = i + 1u;
+        }
+        total += static_cast<double>(tilesOf(g)) * ((g.row_tiles + 1u) / 2u) * kv_heads * unitNs(g);
+    }
+    // One thread block per SM, all of about the same cost.
+    double const share = total / num_sms;
+    std::uint32_t count = 0;
+    std::uint64_t part_rows = 0;
+    auto put = [&](kk_prefix_item const& item) {
+        if (count < max_items) {
+            items[count] = item;
+        }
+        ++count;
+    };
+    for (std::uint32_t i = 0; i < num_groups; ++i) {
+        kk_prefix_group& g = groups[i];
+        std::uint32_t const tiles = tilesOf(g);
+        g.part_row = g.part_count = 0;
+        if (tiles == 0 || g.row_tiles == 0) {
+            continue;
+        }
+        double const want = std::floor(tiles * unitNs(g) / share);
+        std::uint32_t const parts = want < 1. ? 1u : want > tiles ? tiles : static_cast<std::uint32_t>(want);
+        g.part_count = parts;
+        std::uint64_t const rows = std::uint64_t(kv_heads) * parts * g.row_tiles * kTile;
+        if (part_rows + rows > 0xffffffffull) {
+            return KK_EINVAL;
+        }
+        g.part_row = static_cast<std::uint32_t>(part_rows);
+        part_rows += rows;
+        std::uint32_t part = 0, begin = g.desc_offset, before = 0;
+        auto emit = [&](std::uint32_t end, std::uint32_t closed) {
+            for (std::uint32_t h = 0; h < kv_heads; ++h) {
+                for (std::uint32_t r = 0; r < g.row_tiles; r += 2u) {
+                    put(kk_prefix_item{i, h, begin, end, part, static_cast<std::uint16_t>(r),
+                        static_cast<std::uint16_t>(g.row_tiles - r > 1u ? 2u : 1u), closed - before, 0});
+                }
+            }
+            ++part;
+            begin = end;
+            before = closed;
+        };
+        walkTiles(descs, g.desc_offset, g.desc_offset + g.desc_count, [&](std::uint32_t closed, std::uint32_t e) {
+            if (closed == static_cast<std::uint32_t>(std::uint64_t(tiles) * (part + 1u) / parts)) {
+                emit(e, closed);
+            }
+        });
+        emit(g.desc_offset + g.desc_count, tiles);
+    }
+    plan->num_shared = count;
+    if (own_tokens != 0) {
+        double const own_ns = static_cast<double>(own_tokens) * kv_heads * kOwnTokenNs;
+        std::uint32_t ctas = static_cast<std::uint32_t>(std::ceil(own_ns / share));
+        if (count < num_sms && ctas < num_sms - count) {
+            ctas = num_sms - count;
+        }
+        std::uint64_t const warps = std::uint64_t(ctas) * kSoftWarps;
+        std::uint64_t per_task = (own_tokens * kv_heads + warps - 1u) / warps;
+        per_task = per_task < kOwnMinTokens ? kOwnMinTokens : per_task;
+        for (std::uint32_t b = 0; b < num_lanes; ++b) {
+            kk_attn_lane& ln = lanes[b];
+            std::uint32_t const end = ln.desc_offset + ln.desc_count;
+            std::uint64_t len = 0;
+            for (std::uint32_t e = ln.desc_offset; e < end; ++e) {
+                len += 8u * groupsOf(descs[e]);
+            }
+            if (len == 0) {
+                continue;
+            }
+            std::uint64_t const parts = (len + per_task - 1u) / per_task;
+            std::uint64_t const goal = (len + parts - 1u) / parts;
+            ln.item_offset = static_cast<std::uint32_t>(part_rows);
+            std::uint32_t begin = ln.desc_offset;
+            std::uint64_t held = 0;
+            for (std::uint32_t e = ln.desc_offset; e < end; ++e) {
+                held += 8u * groupsOf(descs[e]);
+                if (held >= goal || e + 1u == end) {
+                    for (std::uint32_t h = 0; h < kv_heads; ++h) {
+                        put(kk_prefix_item{b, h, begin, e + 1u, ln.item_count, 0, 0, 0, 0});
+                    }
+                    ++ln.item_count;
+                    part_rows += q_heads;
+                    if (part_rows > 0xffffffffull) {
+                        return KK_EINVAL;
+                    }
+                    begin = e + 1u;
+                    held = 0;
+                }
+            }
+        }
+        std::uint32_t const tasks = count - plan->num_shared;
+        std::uint32_t const per_cta = (tasks + ctas - 1u) / ctas;
+        plan->tasks_per_cta = per_cta < kSoftWarps ? kSoftWarps : per_cta;
+    }
+    plan->num_items = count;
+    plan->part_rows = part_rows;
+    return 0;
+}
+
+uint64_t kk_prefix_attention_workspace_bytes(const kk_prefix_plan* plan)
+{
+    return plan == nullptr ? 0 : plan->part_rows * (kk::kHeadDim * 4u + 8u);
+}
+
+int kk_prefix_attention(const kk_prefix_attn_desc* d, void* stream)
+{
+    using namespace kk;
+    auto misaligned = [](void const* p) { return p == nullptr || (reinterpret_cast<std::uintptr_t>(p) & 15u) != 0; };
+    if (d == nullptr || d->pools.head_dim != kHeadDim || d->layer >= d->pools.layers
+        || !headsServed(d->q_heads, d->pools.kv_heads) || !microPageTokensValid(d->pools)
+        || d->pools.layers > (1u << 24) || d->plan.q_heads != d->q_heads || d->plan.kv_heads != d->pools.kv_heads
+        || !(d->scale > 0.f) || !std::isfinite(d->scale) || d->plan.num_shared > d->plan.num_items
+        || d->plan.tasks_per_cta == 0 || d->plan.part_rows > 0xffffffffull) {
+        return KK_EINVAL;
+    }
+    if (d->plan.num_lanes == 0) {
+        return 0;
+    }
+    std::uint64_t const q_row = std::uint64_t(d->q_heads) * kHeadDim;
+    if (d->lanes == nullptr || misaligned(d->query) || misaligned(d->output) || d->query_stride % 8 != 0
+        || d->output_stride % 8 != 0 || d->query_stride < q_row || d->output_stride < q_row
+        || (d->plan.num_groups != 0 && d->groups == nullptr)
+        || (d->plan.num_items != 0 && (d->items == nullptr || d->descs == nullptr))
+        || (d->plan.num_descs != 0 && (reinterpret_cast<std::uintptr_t>(d->descs) & 3u) != 0)
+        || (d->plan.part_rows != 0
+            && (misaligned(d->workspace)
+                || d->workspace_bytes < kk_prefix_attention_workspace_bytes(&d->plan)))) {
+        return KK_EINVAL;
+    }
+    std::uint64_t const threads = std::uint64_t(d->plan.num_lanes) * d->q_heads * 16u;
+    if (threads > 0xffffffffull) {
+        return KK_EINVAL;
+    }
+    Args a{};
+    a.micro_cap = microPageTokens(d->pools);
+    a.micro = static_cast<__half const*>(d->pools.micro);
+    a.extent = static_cast<__half const*>(d->pools.extent);
+    std::uint64_t const row = std::uint64_t(d->pools.kv_heads) * kHeadDim;
+    a.micro_page = std::uint64_t(d->pools.layers) * 2u * a.micro_cap * row;
+    a.extent_page = std::uint64_t(d->pools.layers) * 2u * 64u * row;
+    a.micro_slots = d->pools.micro == nullptr ? 0 : d->pools.micro_capacity;
+    a.extent_slots = d->pools.extent == nullptr ? 0 : d->pools.extent_capacity;
+    if ((a.micro_slots != 0 && misaligned(a.micro)) || (a.extent_slots != 0 && misaligned(a.extent))) {
+        return KK_EINVAL;
+    }
+    a.layer = d->layer;
+    a.kv_heads = d->pools.kv_heads;
+    a.group = d->q_heads / d->pools.kv_heads;
+    a.plan = d->plan;
+    a.descs = d->descs;
+    a.lanes = d->lanes;
+    a.groups = d->groups;
+    a.items = d->items;
+    a.query = reinterpret_cast<__half const*>(d->query);
+    a.output = reinterpret_cast<__half*>(d->output);
+    a.query_stride = d->query_stride;
+    a.output_stride = d->output_stride;
+    a.scale_log2 = d->scale * 1.4426950408889634f;
+    a.part_o = static_cast<float*>(d->workspace);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + d->plan.part_rows * kHeadDim);
+    cudaStream_t const s = static_cast<cudaStream_t>(stream);
+    if (d->plan.num_items != 0) {
+        cudaError_t const e = allowSharedMemory();
+        if (e != cudaSuccess) {
+            return static_cast<int>(e);
+        }
+        Maps maps{};
+        std::uint32_t const heads = d->pools.kv_heads;
+        if (d->plan.num_shared != 0) {
+            // A pool without pages keeps an empty map: no descriptor selects it.
+            if ((a.micro_slots != 0
+                    && (!encodePageHeadMap(&maps.micro8, a.micro, a.micro_slots, a.micro_cap, d->pools.layers, heads, 8)
+                        || !encodePageHeadMap(&maps.micro, a.micro, a.micro_slots, a.micro_cap, d->pools.layers, heads,
+                            a.micro_cap)))
+                || (a.extent_slots != 0
+                    && (!encodePageHeadMap(&maps.extent8, a.extent, a.extent_slots, 64, d->pools.layers, heads, 8)
+                        || !encodePageHeadMap(&maps.extent, a.extent, a.extent_slots, 64, d->pools.layers, heads,
+                            64)))) {
+                return KK_EINVAL;
+            }
+        }
+        std::uint32_t const own = d->plan.num_items - d->plan.num_shared;
+        std::uint64_t const grid = d->plan.num_shared
+            + (std::uint64_t(own) + d->plan.tasks_per_cta - 1u) / d->plan.tasks_per_cta;
+        if (grid > 0x7fffffffull) {
+            return KK_EINVAL;
+        }
+        int const rc = static_cast<int>(launch(a.group <= 8u ? prefix_attention_kernel<1> : prefix_attention_kernel<2>,
+            dim3(static_cast<unsigned>(grid)), dim3(kThreads), kSmemBytes, s, 1, maps, a));
+        if (rc != 0) {
+            return rc;
+        }
+    }
+    // The joining launch is always a programmatic dependent of the first: its
+    // blocks are set up while the last items run, and wait for their end.
+    bool const pdl = g_pdl_enabled;
+    g_pdl_enabled = true;
+    int const rc = static_cast<int>(launch(prefix_join_kernel,
+        dim3(static_cast<unsigned>((threads + kJoinThreads - 1u) / kJoinThreads)), dim3(kJoinThreads), 0, s, 1, a));
+    g_pdl_enabled = pdl;
+    return rc;
+}
+
+} // extern "C"

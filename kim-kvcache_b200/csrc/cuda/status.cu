@@ -30,6 +30,7 @@ int attentionTmaStatus(cudaStream_t stream);
 int pagesStatus(cudaStream_t stream);
 int gemmStatus(cudaStream_t stream);
 int logitsStatus(cudaStream_t stream);
+int prefixStatus(cudaStream_t stream);
 
 } // namespace kk
 
@@ -39,7 +40,7 @@ int kk_device_status(void* stream)
 {
     cudaStream_t const s = static_cast<cudaStream_t>(stream);
     int const codes[] = {kk::attentionStatus(s), kk::attentionTmaStatus(s), kk::pagesStatus(s),
-        kk::gemmStatus(s), kk::logitsStatus(s)};
+        kk::gemmStatus(s), kk::logitsStatus(s), kk::prefixStatus(s)};
     for (int c : codes) {
         if (c != 0) {
             return c;
