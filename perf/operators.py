@@ -208,8 +208,8 @@ def _prepare_append(c, rng, gen):
 
 def _kk_pools(kk, s, c):
     base = s["storage"].data_ptr()
-    return kk.KvPools(base, base + 2 * s["n_micro"] * s["row"] if s["extent"] else 0, s["micro"], s["extent"],
-                      s["layers"], c["kv_heads"], s["head_dim"], c["page"])
+    return kk.KvPools(base, base + 2 * int(s["n_micro"]) * s["row"] if s["extent"] else 0, int(s["micro"]),
+                      int(s["extent"]), s["layers"], c["kv_heads"], s["head_dim"], c["page"])
 
 
 def _table(tokens, page, pages):
