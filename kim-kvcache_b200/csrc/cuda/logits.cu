@@ -1,19 +1,29 @@
 // K7 — penalties, biases and grammar masks on FP32 logits, and the greedy
 // token, in one pass over the logits.
 //
-// One thread-block cluster takes one row; each of its CTAs owns a contiguous
-// slice of the vocabulary with one 32-bit word per token in shared memory:
-// how often the row's output named the token (low 30 bits), whether the
-// history names it at all, and whether a bias does. The history is read once
-// for the whole row: every CTA reads its share of it and adds each token to
-// the owner's word through distributed shared memory. Counts are integers, so
-// the order in which they arrive changes nothing. Then every CTA streams its
-// slice of the logits, 16 bytes a thread at a time (rows that start on odd
-// addresses included), and keeps the highest allowed one; the cluster's
-// winners meet in its first CTA.
+// One thread-block cluster takes one row; its CTAs own the vocabulary in turn,
+// 256 tokens at a time (text names low ids far more often than high ones:
+// with one contiguous slice per CTA the first one had half of the history). A CTA
+//  1. counts, in shared memory, what of the row's history is its own (every CTA
+//     reads the whole history) and lists each token at its first occurrence;
+//  2. replaces the counts of the listed tokens by their penalised logits;
+//  3. adds the biases to those, or to the plain logits;
+//  4. streams its logits, 16 bytes a thread at a time (rows that start on odd
+//     addresses included), takes the replaced ones from shared memory, applies
+//     the mask and keeps the highest; the cluster's winners meet in its first
+//     CTA.
+// Few tokens of a vocabulary are ever penalised, but few warps of the stream
+// meet none, so step 4 computes nothing for them. Counts are integers and a
+// replaced logit has one writer, so the order of threads changes nothing.
 //
-// HBM bounds it: 4 bytes read and 4 written per logit. The slice is asked into
-// L2 at the start, so that DRAM works while the history is counted.
+// HBM bounds it: 4 bytes read and 4 written per logit. The CTA's logits are
+// asked into L2 at the start, so that DRAM works while the history is counted.
+// Measured on 256 rows of 128,000 logits with about 10,000 tokens of history
+// each (262 MB, 40 us at the measured copy rate): @@LARGE@@; 132 us
+// with the penalties inside the stream (82 instructions a logit); 150 us with
+// contiguous slices and a second pass over the history in place of the list;
+// 200 us with each history read once and counted through distributed shared
+// memory.
 #include "../../../include/kk_kernels.h"
 #include "kernels_internal.h"
 #include "launch.cuh"
@@ -26,31 +36,28 @@ __device__ unsigned int g_logits_status;
 
 namespace {
 
-constexpr int kThreads = 512;
+constexpr std::uint32_t kThreads = 384;
 constexpr std::uint32_t kMaxCluster = 8;
-constexpr std::uint32_t kSeen = 0x80000000u;    // the token is in the history
-constexpr std::uint32_t kBiased = 0x40000000u;  // the token has a bias
-constexpr std::uint32_t kCount = 0x3fffffffu;   // its occurrences in the output
-constexpr std::uint32_t kVecs = 4;              // 16-byte loads in flight per thread
-constexpr std::uint32_t kMaxSliceBytes = 200u * 1024u;
+constexpr std::uint32_t kBlock = 256;          // consecutive tokens of one CTA
+constexpr std::uint32_t kVecs = 2;             // 16-byte loads in flight per thread
+constexpr std::uint32_t kQuads = 4;            // 16-byte history loads in flight per thread
+constexpr std::uint32_t kPrompt = 0x80000000u; // the prompt names the token; below: occurrences in the output
+constexpr std::uint32_t kListed = 2048;        // tokens listed at most; with more, step 2 looks at every word
+constexpr std::uint32_t kMaxSharedBytes = 222u * 1024u;
 
 struct LogitsArgs {
     kk_logits_desc d;
-    std::uint32_t cluster;  // CTAs per row
-    std::uint32_t slice;    // tokens per CTA, a multiple of 32
+    std::uint32_t cluster_log2;  // CTAs per row
+    // Places in shared memory, in 32-bit words; a place of a token is its
+    // number among the CTA's own (the first `capacity`), or capacity + token
+    // for the up to three tokens before the row's first 16-byte step.
+    std::uint32_t capacity;
+    std::uint32_t touched_at;    // a bit per place, set: the word is the token's new logit
+    std::uint32_t mask_at;       // a bit per place, set: allowed
+    std::uint32_t list_at;       // 16-bit places
 };
 
 __device__ __forceinline__ void report(unsigned int code) { atomicCAS(&g_logits_status, kErrNone, code); }
-
-__device__ __forceinline__ void red_add_cluster(std::uint32_t addr, std::uint32_t v)
-{
-    asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
-}
-
-__device__ __forceinline__ void red_or_cluster(std::uint32_t addr, std::uint32_t v)
-{
-    asm volatile("red.relaxed.cluster.shared::cluster.or.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
-}
 
 __device__ __forceinline__ void cluster_arrive()
 {
@@ -79,272 +86,352 @@ __device__ __forceinline__ std::uint64_t candidate(float x, std::uint32_t id)
     return (std::uint64_t(order) << 32) | (0xffffffffu - id);
 }
 
-__global__ void __launch_bounds__(kThreads) logits_process_kernel(const __grid_constant__ LogitsArgs a)
+__global__ void __launch_bounds__(kThreads, 3) logits_process_kernel(const __grid_constant__ LogitsArgs a)
 {
     extern __shared__ __align__(16) std::uint32_t s_words[];
     __shared__ std::uint64_t s_best[kThreads / 32];
     __shared__ std::uint64_t s_cluster[kMaxCluster];
+    __shared__ std::uint32_t s_listed;
     pdl_launch_dependents();
     pdl_wait();
     kk_logits_desc const& d = a.d;
     std::uint32_t const tid = threadIdx.x;
-    std::uint32_t const rank = a.cluster > 1 ? cluster_rank() : 0u;
-    std::uint32_t const row = blockIdx.x / a.cluster;
-    std::uint32_t const begin = rank * a.slice < d.vocab ? rank * a.slice : d.vocab;
-    std::uint32_t const end = d.vocab - begin < a.slice ? d.vocab : begin + a.slice;
-    float const* in = d.logits + row * d.logits_stride;
-    float* out = d.out != nullptr ? d.out + row * d.out_stride : nullptr;
-    // 16-byte steps of logits start at body (slices start on whole 128-byte
-    // steps from the row's start, so the row's misfit is every slice's).
-    std::uint32_t const misfit = static_cast<std::uint32_t>(reinterpret_cast<std::uintptr_t>(in) >> 2) & 3u;
+    std::uint32_t const lc = a.cluster_log2;
+    std::uint32_t const rank = blockIdx.x & ((1u << lc) - 1u);
+    std::uint32_t const row = blockIdx.x >> lc;
+    std::uint32_t const vocab = d.vocab;
+    float const* const in = d.logits + row * d.logits_stride;
+    float* const out = d.out != nullptr ? d.out + row * d.out_stride : nullptr;
     bool const same_phase = out == nullptr
         || ((reinterpret_cast<std::uintptr_t>(out) ^ reinterpret_cast<std::uintptr_t>(in)) & 15u) == 0;
-    std::uint32_t head = (4u - misfit) & 3u;
-    head = head < end - begin ? head : end - begin;
-    std::uint32_t const vecs = (end - begin - head) / 4u;
-    std::uint32_t const body = begin + head;
-    // Words are shifted so that a 16-byte step of logits meets a 16-byte step
-    // of words; the shift is the row's, the same in every CTA of the cluster.
-    std::uint32_t const shift = misfit;
-    std::uint32_t* const words = s_words + shift;  // word of token v: words[v - begin]
+    // Tokens before the first 16-byte step; the first CTA's.
+    std::uint32_t head = (4u - static_cast<std::uint32_t>(reinterpret_cast<std::uintptr_t>(in) >> 2)) & 3u;
+    head = head < vocab ? head : vocab;
+    std::uint32_t const body = vocab - head;
+    std::uint32_t const all_blocks = (body + kBlock - 1u) / kBlock;
+    std::uint32_t const blocks = all_blocks > rank ? ((all_blocks - 1u - rank) >> lc) + 1u : 0u;
+    // Place <-> token, behind the head.
+    auto token_of = [&](std::uint32_t at) {
+        return head + ((((at / kBlock) << lc) + rank) * kBlock) + at % kBlock;
+    };
+    std::uint32_t const owner_mask = ((1u << lc) - 1u) * kBlock;
+    std::uint32_t const owner = rank * kBlock;
+    auto owned = [&](std::uint32_t v) { return v - head < body && ((v - head) & owner_mask) == owner; };
+    auto place_of = [&](std::uint32_t v) {
+        std::uint32_t const u = v - head;
+        return ((u / kBlock) >> lc) * kBlock + u % kBlock;
+    };
+    auto in_head = [&](std::uint32_t v) { return v < head && rank == 0; };
 
-    if (tid == 0 && vecs != 0) {
-        l2_prefetch_bulk(in + body, vecs * 16u);
+    // ---- everything that can be asked for at once: logits, the row's lists
+    for (std::uint32_t i = tid; i < blocks; i += kThreads) {
+        std::uint32_t const v = token_of(i * kBlock);
+        std::uint32_t const n = (vocab - v < kBlock ? vocab - v : kBlock) / 4u;
+        if (n != 0) {
+            l2_prefetch_bulk(in + v, n * 16u);
+        }
     }
-
-    // ---- the row's lists
+    std::uint32_t* const s_touched = s_words + a.touched_at;
+    if (a.touched_at != 0) {  // the call has a history or biases
+        if (d.history_offsets != nullptr) {
+            for (std::uint32_t i = tid; i <= a.capacity / 4u; i += kThreads) {
+                reinterpret_cast<uint4*>(s_words)[i] = make_uint4(0, 0, 0, 0);
+            }
+        }
+        for (std::uint32_t i = tid; i <= a.capacity / 32u; i += kThreads) {
+            s_touched[i] = 0;
+        }
+        if (tid == 0) {
+            s_listed = 0;
+        }
+    }
     float rep = 1.f, pres = 0.f, freq = 0.f;
-    std::uint32_t h0 = 0, h1 = 0, prompt = 0;
+    std::uint32_t h0 = 0, h1 = 0, prompt = 0, b0 = 0, b1 = 0, mask_row = row;
     if (d.history_offsets != nullptr) {
+        h0 = d.history_offsets[row];
+        h1 = d.history_offsets[row + 1];
         rep = d.repetition != nullptr ? d.repetition[row] : 1.f;
         pres = d.presence != nullptr ? d.presence[row] : 0.f;
         freq = d.frequency != nullptr ? d.frequency[row] : 0.f;
-        if (rep != 1.f || pres != 0.f || freq != 0.f) {
-            h0 = d.history_offsets[row];
-            h1 = d.history_offsets[row + 1];
-            if (h1 < h0 || h1 > d.history_size) {
-                if (tid == 0) {
-                    report(kErrBadArgument);
-                }
-                h0 = h1 = 0;
-            }
-            prompt = d.prompt_counts != nullptr ? d.prompt_counts[row] : 0u;
-        }
+        prompt = d.prompt_counts != nullptr ? d.prompt_counts[row] : 0u;
     }
-    std::uint32_t b0 = 0, b1 = 0;
     if (d.bias_offsets != nullptr) {
         b0 = d.bias_offsets[row];
         b1 = d.bias_offsets[row + 1];
-        if (b1 < b0 || b1 > d.bias_size) {
-            if (tid == 0) {
-                report(kErrBadArgument);
-            }
-            b0 = b1 = 0;
-        }
     }
-    bool const penal = h1 > h0;
-    bool const biased = b1 > b0;
+    if (d.mask != nullptr && d.mask_rows != nullptr) {
+        mask_row = d.mask_rows[row];
+    }
+    bool bad = false;
+    if (h1 < h0 || h1 > d.history_size) {
+        bad = true;
+        h0 = h1 = 0;
+    }
+    if (rep == 1.f && pres == 0.f && freq == 0.f) {
+        h0 = h1 = 0;  // the history changes nothing
+    }
+    if (b1 < b0 || b1 > d.bias_size) {
+        bad = true;
+        b0 = b1 = 0;
+    }
     std::uint32_t const* mask = nullptr;
     bool blocked = false;  // a mask row outside the masks: nothing is allowed
     if (d.mask != nullptr) {
-        std::uint32_t const m = d.mask_rows != nullptr ? d.mask_rows[row] : row;
-        if (m < d.num_masks) {
-            mask = d.mask + std::uint64_t(m) * d.mask_stride;
-        } else if (m != KK_NO_MASK || d.mask_rows == nullptr) {
-            blocked = true;
-            if (tid == 0) {
-                report(kErrBadArgument);
-            }
+        if (mask_row < d.num_masks) {
+            mask = d.mask + std::uint64_t(mask_row) * d.mask_stride;
+        } else if (mask_row != KK_NO_MASK || d.mask_rows == nullptr) {
+            bad = blocked = true;
         }
     }
-
+    if (bad && tid == 0) {
+        report(kErrBadArgument);
+    }
+    bool const penal = h1 > h0;
+    bool const use_words = penal || b1 > b0;
+    // The first bias of each thread, and the logit that it changes.
+    std::uint32_t bias_token = 0, bias_next = 0xffffffffu;
+    float bias_value = 0.f, bias_logit = 0.f;
+    auto load_bias = [&](std::uint32_t i) {
+        bias_token = d.bias_tokens[i];
+        bias_next = i + 1 < b1 ? d.bias_tokens[i + 1] : 0xffffffffu;
+        bias_value = d.bias_values[i];
+        bias_logit = owned(bias_token) || in_head(bias_token) ? in[bias_token] : 0.f;
+    };
+    if (b0 + tid < b1) {
+        load_bias(b0 + tid);
+    }
     // Before a CTA writes into another one's shared memory, all of the cluster
-    // have started: with a history the barriers around its count see to
-    // that, without one this pair does (its wait stands at the end).
-    bool const greet = a.cluster > 1 && !penal && d.tokens != nullptr;
-    if (greet) {
+    // have started: they say so here and ask at the end.
+    if (lc != 0 && d.tokens != nullptr) {
         cluster_arrive();
     }
 
-    // ---- words
-    if (penal || biased) {
-        std::uint32_t const n = (end - begin + shift + 3u) / 4u;
-        for (std::uint32_t i = tid; i < n; i += kThreads) {
-            reinterpret_cast<uint4*>(s_words)[i] = make_uint4(0, 0, 0, 0);
-        }
-        if (penal && a.cluster > 1) {
-            cluster_sync();
-        } else {
-            __syncthreads();
-        }
-        for (std::uint32_t i = b0 + tid; i < b1; i += kThreads) {
-            std::uint32_t const v = d.bias_tokens[i];
-            if (v >= begin && v < end) {
-                atomicOr(&words[v - begin], kBiased);
-            }
-            if (i + 1 < b1 && d.bias_tokens[i + 1] < v) {
-                report(kErrBadArgument);
-            }
-        }
-        if (penal) {
-            std::uint64_t const len = h1 - h0;
-            std::uint32_t const lo = static_cast<std::uint32_t>(len * rank / a.cluster);
-            std::uint32_t const hi = static_cast<std::uint32_t>(len * (rank + 1u) / a.cluster);
-            for (std::uint32_t i = lo + tid; i < hi; i += kThreads) {
-                std::uint32_t const v = d.history[std::uint64_t(h0) + i];
-                if (v >= d.vocab) {
-                    continue;
-                }
-                std::uint32_t const owner = v / a.slice;
-                std::uint32_t* const word = &words[v - owner * a.slice];
-                std::uint32_t const addr = a.cluster > 1 ? cluster_map(word, owner) : smem_u32(word);
-                if (i < prompt) {
-                    red_or_cluster(addr, kSeen);
-                } else {
-                    red_add_cluster(addr, 1u);
-                }
-            }
-        }
-        if (penal && a.cluster > 1) {
-            cluster_sync();
-        } else {
-            __syncthreads();
+    std::uint32_t* const s_mask = s_words + a.mask_at;
+    std::uint16_t* const s_list = reinterpret_cast<std::uint16_t*>(s_words + a.list_at);
+    if (mask != nullptr) {
+        // Brought to the places' order; bits behind the vocabulary are never asked for.
+        std::uint32_t const last = (vocab - 1u) / 32u;
+        for (std::uint32_t i = tid; i < blocks * (kBlock / 32u); i += kThreads) {
+            std::uint32_t const v = token_of(i * 32u);
+            std::uint32_t const w = v / 32u < last ? v / 32u : last;
+            s_mask[i] = __funnelshift_r(__ldg(mask + w), __ldg(mask + (w < last ? w + 1u : last)), v & 31u);
         }
     }
+    __syncthreads();
 
-    // ---- the slice
-    auto penalised = [&](float x, std::uint32_t w) {
-        if ((w & ~kBiased) != 0) {
-            x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
-            if ((w & kCount) != 0) {
-                x = __fsub_rn(x, __fmul_rn(freq, static_cast<float>(w & kCount)));
-                x = __fsub_rn(x, pres);
+    // ---- the history and the biases
+    auto replace = [&](std::uint32_t at, float x) {
+        s_words[at] = __float_as_uint(x);
+        atomicOr(&s_touched[at / 32u], 1u << (at % 32u));
+    };
+    if (penal) {
+        auto count = [&](std::uint32_t at, std::uint32_t i) {
+            std::uint32_t const before = i < prompt ? atomicOr(&s_words[at], kPrompt) : atomicAdd(&s_words[at], 1u);
+            if (before == 0) {
+                std::uint32_t const n = atomicAdd(&s_listed, 1u);
+                if (n < kListed) {
+                    s_list[n] = static_cast<std::uint16_t>(at);
+                }
+            }
+        };
+        std::uint32_t const* const text = d.history + h0;
+        std::uint32_t const len = h1 - h0;
+        std::uint32_t const lead = (4u - static_cast<std::uint32_t>(reinterpret_cast<std::uintptr_t>(text) >> 2)) & 3u;
+        std::uint32_t const from = lead < len ? lead : len;
+        std::uint32_t const quads = (len - from) / 4u;
+        for (std::uint32_t q0 = tid; q0 < quads; q0 += kThreads * kQuads) {
+            uint4 ahead[kQuads];
+#pragma unroll
+            for (std::uint32_t k = 0; k < kQuads; ++k) {
+                std::uint32_t const q = q0 + k * kThreads;
+                if (q < quads) {
+                    ahead[k] = __ldg(reinterpret_cast<uint4 const*>(text + from) + q);
+                }
+            }
+#pragma unroll
+            for (std::uint32_t k = 0; k < kQuads; ++k) {
+                std::uint32_t const q = q0 + k * kThreads;
+                if (q >= quads) {
+                    break;
+                }
+                uint4 const t = ahead[k];
+                std::uint32_t mine = (owned(t.x) ? 1u : 0u) | (owned(t.y) ? 2u : 0u) | (owned(t.z) ? 4u : 0u)
+                    | (owned(t.w) ? 8u : 0u);
+                if (head != 0) {
+                    std::uint32_t const v[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+                    for (std::uint32_t e = 0; e < 4u; ++e) {
+                        if (in_head(v[e])) {
+                            count(a.capacity + v[e], from + q * 4u + e);
+                        }
+                    }
+                }
+                // One token per thread and turn: about two turns a warp, not four.
+                while (mine != 0) {
+                    std::uint32_t const e = __ffs(mine) - 1u;
+                    mine &= mine - 1u;
+                    std::uint32_t const v = e < 2u ? (e == 0 ? t.x : t.y) : (e == 2u ? t.z : t.w);
+                    count(place_of(v), from + q * 4u + e);
+                }
             }
         }
-        return x;
+        std::uint32_t const edge = tid < from ? tid : from + quads * 4u + (tid - from);
+        if (edge < len && tid < from + 3u) {
+            std::uint32_t const v = text[edge];
+            if (owned(v)) {
+                count(place_of(v), edge);
+            } else if (in_head(v)) {
+                count(a.capacity + v, edge);
+            }
+        }
+        __syncthreads();
+        auto logit_at = [&](std::uint32_t at) { return in[at < a.capacity ? token_of(at) : at - a.capacity]; };
+        auto penalise = [&](std::uint32_t at, float x) {
+            std::uint32_t const n = s_words[at] & ~kPrompt;
+            x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
+            if (n != 0) {
+                x = __fsub_rn(x, __fmul_rn(freq, static_cast<float>(n)));
+                x = __fsub_rn(x, pres);
+            }
+            replace(at, x);
+        };
+        std::uint32_t const listed = s_listed;
+        if (listed <= kListed) {
+            for (std::uint32_t i0 = tid; i0 < listed; i0 += kThreads * kQuads) {
+                std::uint32_t at[kQuads];
+                float x[kQuads];
+#pragma unroll
+                for (std::uint32_t k = 0; k < kQuads; ++k) {
+                    std::uint32_t const i = i0 + k * kThreads;
+                    at[k] = i < listed ? s_list[i] : 0u;
+                    x[k] = i < listed ? logit_at(at[k]) : 0.f;
+                }
+#pragma unroll
+                for (std::uint32_t k = 0; k < kQuads; ++k) {
+                    if (i0 + k * kThreads < listed) {
+                        penalise(at[k], x[k]);
+                    }
+                }
+            }
+        } else {
+            for (std::uint32_t i = tid; i < blocks * kBlock + head; i += kThreads) {
+                std::uint32_t const at = i < blocks * kBlock ? i : a.capacity + (i - blocks * kBlock);
+                if (s_words[at] != 0) {
+                    penalise(at, logit_at(at));
+                }
+            }
+        }
+        __syncthreads();
+    }
+    for (std::uint32_t i = b0 + tid; i < b1; i += kThreads) {
+        if (i != b0 + tid) {
+            load_bias(i);
+        }
+        std::uint32_t const v = bias_token;
+        if (bias_next < v) {
+            report(kErrBadArgument);
+        }
+        bool const low = in_head(v);
+        if ((low || owned(v)) && bias_next != v) {
+            std::uint32_t const at = low ? a.capacity + v : place_of(v);
+            bool const replaced = (s_touched[at / 32u] >> (at % 32u) & 1u) != 0;
+            replace(at, __fadd_rn(replaced ? __uint_as_float(s_words[at]) : bias_logit, bias_value));
+        }
+    }
+    if (b1 > b0) {
+        __syncthreads();
+    }
+
+    // ---- the logits
+    // A thread meets its tokens in ascending order, so a strict comparison
+    // keeps the lowest id of equal logits; NaN and -inf never pass it.
+    float top = -INFINITY;
+    std::uint32_t top_id = 0;
+    auto offer = [&](float x, std::uint32_t v) {
+        if (x > top) {
+            top = x;
+            top_id = v;
+        }
     };
-    auto allowed4 = [&](std::uint32_t v) -> std::uint32_t {  // bits of tokens v .. v + 3
-        if (blocked) {
-            return 0u;
-        }
-        if (mask == nullptr) {
-            return 15u;
-        }
-        std::uint32_t const w0 = mask[v / 32u];
-        std::uint32_t const last = v + 3u < d.vocab ? v + 3u : d.vocab - 1u;
-        std::uint32_t const w1 = mask[last / 32u];
-        return __funnelshift_r(w0, w1, v & 31u) & 15u;
-    };
-    bool const use_words = penal || biased;
-    std::uint64_t best = 0;
-    auto one = [&](std::uint32_t v) {
-        std::uint32_t const w = use_words ? words[v - begin] : 0u;
-        if (w & kBiased) {
-            return;
-        }
-        float x = penalised(in[v], w);
-        x = (allowed4(v) & 1u) != 0 ? x : -INFINITY;
+    auto bits_of = [&](std::uint32_t const* bits, std::uint32_t at) { return bits[at / 32u] >> (at % 32u); };
+    auto one = [&](std::uint32_t at, std::uint32_t v, bool allowed) {
+        float x = use_words && (bits_of(s_touched, at) & 1u) != 0 ? __uint_as_float(s_words[at]) : in[v];
+        x = allowed && !blocked ? x : -INFINITY;
         if (out != nullptr) {
             out[v] = x;
         }
-        std::uint64_t const c = candidate(x, v);
-        best = c > best ? c : best;
+        offer(x, v);
     };
-    if (tid < head) {
-        one(begin + tid);
+    if (rank == 0 && tid < head) {
+        one(a.capacity + tid, tid, mask == nullptr || (mask[0] >> tid & 1u) != 0);
     }
-    {
-        std::uint32_t const v = body + vecs * 4u + tid;  // at most 3 tokens
-        if (v < end) {
-            one(v);
-        }
-    }
-    for (std::uint32_t i0 = tid; i0 < vecs; i0 += kThreads * kVecs) {
+    std::uint32_t const steps = blocks * (kBlock / 4u);
+    for (std::uint32_t i0 = tid; i0 < steps; i0 += kThreads * kVecs) {
         float4 x[kVecs];
 #pragma unroll
         for (std::uint32_t k = 0; k < kVecs; ++k) {
             std::uint32_t const i = i0 + k * kThreads;
-            if (i < vecs) {
-                x[k] = reinterpret_cast<float4 const*>(in + body)[i];
+            std::uint32_t const v = token_of(i * 4u);
+            if (i < steps && v + 4u <= vocab) {
+                x[k] = *reinterpret_cast<float4 const*>(in + v);
             }
         }
 #pragma unroll
         for (std::uint32_t k = 0; k < kVecs; ++k) {
             std::uint32_t const i = i0 + k * kThreads;
-            if (i >= vecs) {
-                break;
-            }
-            std::uint32_t const v = body + i * 4u;
-            std::uint32_t const allow = allowed4(v);
-            float y[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
-            std::uint32_t flagged = 0;
-            if (use_words) {
-                uint4 const w = *reinterpret_cast<uint4 const*>(&words[v - begin]);
-                if ((w.x | w.y | w.z | w.w) != 0) {
-                    y[0] = penalised(y[0], w.x);
-                    y[1] = penalised(y[1], w.y);
-                    y[2] = penalised(y[2], w.z);
-                    y[3] = penalised(y[3], w.w);
-                    flagged = (w.x | w.y | w.z | w.w) & kBiased;
-                    if (flagged) {
-                        // Biased tokens are left to the pass over the biases.
-                        std::uint32_t const ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            if ((ws[e] & kBiased) == 0) {
-                                float const z = (allow >> e & 1u) != 0 ? y[e] : -INFINITY;
-                                if (out != nullptr) {
-                                    out[v + e] = z;
-                                }
-                                std::uint64_t const c = candidate(z, v + e);
-                                best = c > best ? c : best;
-                            }
-                        }
-                    }
-                }
-            }
-            if (flagged) {
+            std::uint32_t const at = i * 4u;
+            std::uint32_t const v = token_of(at);
+            if (i >= steps || v >= vocab) {
                 continue;
             }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                y[e] = (allow >> e & 1u) != 0 ? y[e] : -INFINITY;
-                std::uint64_t const c = candidate(y[e], v + e);
-                best = c > best ? c : best;
+            std::uint32_t allow = blocked ? 0u : 15u;
+            if (mask != nullptr) {
+                allow = bits_of(s_mask, at);
+            }
+            if (v + 4u > vocab) {  // the last, partial step
+                for (std::uint32_t e = 0; v + e < vocab; ++e) {
+                    one(at + e, v + e, (allow >> e & 1u) != 0);
+                }
+                continue;
+            }
+            if (use_words) {
+                std::uint32_t const replaced = bits_of(s_touched, at) & 15u;
+                if (replaced != 0) {
+                    uint4 const w = *reinterpret_cast<uint4 const*>(&s_words[at]);
+                    x[k].x = (replaced & 1u) != 0 ? __uint_as_float(w.x) : x[k].x;
+                    x[k].y = (replaced & 2u) != 0 ? __uint_as_float(w.y) : x[k].y;
+                    x[k].z = (replaced & 4u) != 0 ? __uint_as_float(w.z) : x[k].z;
+                    x[k].w = (replaced & 8u) != 0 ? __uint_as_float(w.w) : x[k].w;
+                }
+            }
+            x[k].x = (allow & 1u) != 0 ? x[k].x : -INFINITY;
+            x[k].y = (allow & 2u) != 0 ? x[k].y : -INFINITY;
+            x[k].z = (allow & 4u) != 0 ? x[k].z : -INFINITY;
+            x[k].w = (allow & 8u) != 0 ? x[k].w : -INFINITY;
+            if (d.tokens != nullptr) {
+                offer(x[k].x, v);
+                offer(x[k].y, v + 1u);
+                offer(x[k].z, v + 2u);
+                offer(x[k].w, v + 3u);
             }
             if (out != nullptr) {
                 if (same_phase) {
-                    *reinterpret_cast<float4*>(out + v) = make_float4(y[0], y[1], y[2], y[3]);
+                    *reinterpret_cast<float4*>(out + v) = x[k];
                 } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        out[v + e] = y[e];
-                    }
+                    out[v] = x[k].x;
+                    out[v + 1u] = x[k].y;
+                    out[v + 2u] = x[k].z;
+                    out[v + 3u] = x[k].w;
                 }
             }
         }
-    }
-    for (std::uint32_t i = b0 + tid; i < b1; i += kThreads) {
-        std::uint32_t const v = d.bias_tokens[i];
-        if (v < begin || v >= end || (i + 1 < b1 && d.bias_tokens[i + 1] == v)) {
-            continue;
-        }
-        float x = __fadd_rn(penalised(in[v], words[v - begin]), d.bias_values[i]);
-        x = (allowed4(v) & 1u) != 0 ? x : -INFINITY;
-        if (out != nullptr) {
-            out[v] = x;
-        }
-        std::uint64_t const c = candidate(x, v);
-        best = c > best ? c : best;
     }
 
     // ---- the greedy token
     if (d.tokens == nullptr) {
-        return;  // behind the last barrier of the count nothing reads another CTA's words
+        return;
     }
-    if (greet) {
-        cluster_wait();
-    }
+    std::uint64_t best = candidate(top, top_id);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         std::uint64_t const other = __shfl_xor_sync(0xffffffffu, best, o);
@@ -355,18 +442,25 @@ __global__ void __launch_bounds__(kThreads) logits_process_kernel(const __grid_c
     }
     __syncthreads();
     if (tid == 0) {
-        for (int w = 1; w < kThreads / 32; ++w) {
+        for (std::uint32_t w = 1; w < kThreads / 32u; ++w) {
             best = s_best[w] > best ? s_best[w] : best;
         }
-        if (a.cluster > 1) {
+    }
+    if (lc != 0) {
+        cluster_wait();
+        if (tid == 0 && rank != 0) {
             st_cluster_u64(cluster_map(&s_cluster[rank], 0), best);
         }
+        // Only the first CTA waits; the others are done once they said so.
+        __syncwarp();
+        cluster_arrive();
+        if (rank != 0) {
+            return;
+        }
+        cluster_wait();
     }
-    if (a.cluster > 1) {
-        cluster_sync();
-    }
-    if (rank == 0 && tid == 0) {
-        for (std::uint32_t r = 1; r < a.cluster; ++r) {
+    if (tid == 0) {
+        for (std::uint32_t r = 1; r < 1u << lc; ++r) {
             best = s_cluster[r] > best ? s_cluster[r] : best;
         }
         d.tokens[row] = best != 0 ? 0xffffffffu - static_cast<std::uint32_t>(best) : KK_NO_TOKEN;
@@ -383,7 +477,7 @@ cudaError_t allowSharedMemory()
         return e;
     }
     e = cudaFuncSetAttribute(logits_process_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-        static_cast<int>(kMaxSliceBytes + 32u));
+        static_cast<int>(kMaxSharedBytes));
     if (e == cudaSuccess && device < 64) {
         done.fetch_or(std::uint64_t(1) << device, std::memory_order_release);
     }
@@ -427,20 +521,30 @@ extern "C" int kk_logits_process(const kk_logits_desc* d, void* stream)
         return KK_EINVAL;
     }
     bool const words = a.d.history_offsets != nullptr || d->bias_offsets != nullptr;
-    std::uint32_t cluster = 1;
-    while (cluster < kMaxCluster && d->vocab / cluster > 4096u) {
-        cluster *= 2;
+    // CTAs per row: up to eight, none with fewer than 4,096 tokens.
+    while ((1u << a.cluster_log2) < kMaxCluster && (d->vocab >> a.cluster_log2) > 4096u) {
+        ++a.cluster_log2;
     }
-    a.cluster = cluster;
-    a.slice = ((d->vocab + cluster - 1u) / cluster + 31u) / 32u * 32u;
-    std::uint64_t const bytes = words ? std::uint64_t(a.slice + 8u) * 4u : 0u;
-    if (bytes > kMaxSliceBytes || std::uint64_t(d->rows) * cluster > 0x7fffffffu) {
+    std::uint32_t const blocks = (d->vocab + kBlock - 1u) / kBlock;
+    a.capacity = (((blocks - 1u) >> a.cluster_log2) + 1u) * kBlock;
+    std::uint64_t bytes = 0;
+    if (words) {
+        a.touched_at = a.capacity + 4u;
+        a.list_at = a.touched_at + a.capacity / 32u + 1u;
+        bytes = (std::uint64_t(a.list_at) + kListed / 2u) * 4u;
+    }
+    if (d->mask != nullptr) {
+        a.mask_at = static_cast<std::uint32_t>(bytes / 4u);
+        bytes += a.capacity / 8u;
+    }
+    if (bytes > kMaxSharedBytes || (words && a.capacity + 4u > 65536u)
+        || (std::uint64_t(d->rows) << a.cluster_log2) > 0x7fffffffu) {
         return KK_EINVAL;
     }
     cudaError_t const e = allowSharedMemory();
     if (e != cudaSuccess) {
         return static_cast<int>(e);
     }
-    return static_cast<int>(launch(logits_process_kernel, dim3(d->rows * cluster), dim3(kThreads), bytes,
-        static_cast<cudaStream_t>(stream), cluster, a));
+    return static_cast<int>(launch(logits_process_kernel, dim3(d->rows << a.cluster_log2), dim3(kThreads), bytes,
+        static_cast<cudaStream_t>(stream), 1u << a.cluster_log2, a));
 }

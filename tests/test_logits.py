@@ -33,6 +33,7 @@ def valid_desc(kk):
     dict(bias_offsets=16, bias_size=3), dict(bias_offsets=16, bias_size=3, bias_tokens=16),
     dict(mask=16, mask_stride=3, num_masks=2), dict(vocab=(1 << 30) + 1, logits_stride=1 << 31, out_stride=1 << 31),
     dict(vocab=500000, logits_stride=500000, out_stride=500000, bias_offsets=16),
+    dict(vocab=20000000, logits_stride=20000000, out_stride=20000000, mask=16, mask_stride=625000, num_masks=1),
 ], ids=str)
 def test_logits_refuses(kk, change):
     d = valid_desc(kk)
