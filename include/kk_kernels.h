@@ -231,6 +231,10 @@ typedef struct kk_prefix_item {
     uint16_t row_tile;         /* first tile of query rows */
     uint16_t row_tiles;        /* 1 or 2; 0: a lane's own pages */
     uint32_t token_tiles;      /* 128-token tiles of the run */
+    uint32_t part_row;         /* first partial row that the item writes */
+    uint32_t lane_begin;       /* the group's lanes */
+    uint32_t lane_count;
+    uint32_t query_row;        /* the lane's (row_tiles == 0) */
     uint32_t reserved;
 } kk_prefix_item;
 

@@ -397,7 +397,9 @@ class PrefixGroup(C.Structure):
 class PrefixItem(C.Structure):
     _fields_ = [("owner", C.c_uint32), ("kv_head", C.c_uint32), ("desc_begin", C.c_uint32),
                 ("desc_end", C.c_uint32), ("part", C.c_uint32), ("row_tile", C.c_uint16),
-                ("row_tiles", C.c_uint16), ("token_tiles", C.c_uint32), ("reserved", C.c_uint32)]
+                ("row_tiles", C.c_uint16), ("token_tiles", C.c_uint32), ("part_row", C.c_uint32),
+                ("lane_begin", C.c_uint32), ("lane_count", C.c_uint32), ("query_row", C.c_uint32),
+                ("reserved", C.c_uint32)]
 
 
 class PrefixPlan(C.Structure):

@@ -10,27 +10,33 @@
 // (O, row maximum, row sum) and a second, dependent launch joins each query
 // row's partials and rounds once to FP16.
 //
-// Shared item (one block per SM):
+// Shared item (one block per SM), up to two tiles of 128 query rows:
 //  * warp 8 walks the item's descriptors and fills a 4-stage ring with 128-token
 //    tiles of one KV head, K then V, [token][64 dims] with the 128-byte
 //    swizzle (TMA; an 8-token group is one swizzle atom, so pages of any size
-//    meet in a tile). A tile that is not full has the V rows of its invalid
-//    tokens zeroed in shared memory (0 * NaN would be NaN);
-//  * warp 9 issues the tcgen05.mma of both products: Q (TMEM, 128 rows) x K
-//    (shared memory) -> S (TMEM), P (TMEM) x V (shared memory, token rows =
-//    K dimension, i.e. MN-major) -> O (TMEM);
-//  * warps 0-3 and 4-7 are two softmax groups, one thread per query row. With
-//    two row tiles each group has a row tile of its own and both use every
-//    K/V tile; with one row tile they take the token tiles in turn and join at the
-//    end. While one group computes exponentials the tensor core works for
-//    the other.
-// P is handed to the FP16 product as hi + lo halves (p = hi + lo to 2^-21), so
-// that the weights keep FP32 precision as in the per-lane kernel; at 64 dims
-// the tensor core has the time, since the exponentials (16 per SM and clock)
-// bound a full tile: 1,024 clocks of them against 768 of products. The running
-// maximum is only raised, and O only rescaled, when a row's maximum grows by
-// more than 2^8 (P stays below 2^8 and within FP16; the quotient is exact in
-// either case).
+//    meet in a tile; each lane issues the copies of one page). A tile that is
+//    not full has the V rows of its invalid tokens zeroed in shared memory
+//    (0 * NaN would be NaN);
+//  * warp 9 issues the tcgen05.mma of both products: Q (shared memory, 128
+//    rows) x K -> S (TMEM), P (TMEM) x V (shared memory, token rows = K
+//    dimension, i.e. MN-major) -> O (TMEM). Three S tiles take turns: two are
+//    in the hands of the softmax groups while the next scores are formed;
+//  * warps 0-3 and 4-7 are two softmax groups, one thread per query row, each
+//    with its own O. Two row tiles: one group each, every K/V tile for both. One
+//    row tile: the groups take the token tiles in turn and join at the end.
+// P is rounded to FP16 for the second product (the row sums are not): its error,
+// 2^-12 of a weight on average, averages out to about that of the FP16 output.
+// The per-lane kernel adds the product of the low halves; here that second
+// product would be 64 columns wide and so at half of the tensor core's rate.
+// The running maximum is only raised, and O only rescaled, when a row's maximum
+// grows by more than 2^8 (P stays within FP16; the quotient is exact in either
+// case).
+// The exponentials, 16 per SM and clock, bound a K/V tile for 256 rows: 2,048
+// clocks. Measured steps, per such tile: 2.6 us with two groups that waited for
+// each product (or four of half rows), while the products were issued from a branch
+// of one lane (see elect_lane); 1.9 us without that branch; 1.6 us without the
+// low halves; @@TILE@@ with the third S tile. (Four groups in turn over three S
+// tiles: 2.4 us, all three are then in use at once.)
 //
 // A lane's own pages: one warp per (lane, KV head, run of pages), 16-token
 // slices through a private cp.async ring, scores transposed (tokens x heads) on
@@ -50,13 +56,13 @@ namespace {
 
 constexpr std::uint32_t kHeadDim = 64;
 constexpr std::uint32_t kRowBytes = kHeadDim * 2;
-constexpr std::uint32_t kSoftWarps = 8;
+constexpr std::uint32_t kSoftWarps = 8;               // also of a block that serves lanes' own pages
 constexpr std::uint32_t kProducerWarp = 8;
 constexpr std::uint32_t kIssuerWarp = 9;
 constexpr std::uint32_t kThreads = 384;               // three warpgroups; warps 10 and 11 only fill the third
-// A softmax thread holds a row of S (128 values); the third warpgroup gives up
+// A softmax thread holds a row of scores (128 values); the third warpgroup gives up
 // registers for it. The block is launched with kLaunchRegs a thread, and the
-// three shares must fit into that.
+// shares must fit into what was launched.
 constexpr std::uint32_t kLaunchRegs = 168;
 constexpr std::uint32_t kSoftRegs = 216;
 constexpr std::uint32_t kFewRegs = 72;
@@ -64,16 +70,16 @@ static_assert(2 * kSoftRegs + kFewRegs <= 3 * kLaunchRegs, "a share beyond the l
 constexpr std::uint32_t kStages = 4;
 constexpr std::uint32_t kTile = 128;                  // tokens per tile, and query rows per row tile
 constexpr std::uint32_t kSlots = kTile / 8;           // 8-token groups per tile
-constexpr std::uint32_t kHalfStage = kTile * kRowBytes;
-constexpr std::uint32_t kStageBytes = 2 * kHalfStage;
+constexpr std::uint32_t kTileBytes = kTile * kRowBytes;  // K, V or Q
+constexpr std::uint32_t kStageBytes = 2 * kTileBytes;
 constexpr std::uint64_t kAllValid = 0x8888888888888888ull;  // 8 tokens in each of 16 groups
 
 // TMEM columns.
 constexpr std::uint32_t kTmemCols = 512;
-constexpr std::uint32_t kColS = 0;      // two S tiles of 128 columns; P replaces S in place
-constexpr std::uint32_t kColO = 256;    // two O tiles of 64
-constexpr std::uint32_t kColQ = 384;    // two Q tiles of 32 (two FP16 per column)
-constexpr std::uint32_t kColPLo = 64;   // low halves of P, from the start of P
+constexpr std::uint32_t kSTiles = 3;
+constexpr std::uint32_t kColS = 0;      // S tiles of 128 columns
+constexpr std::uint32_t kColO = 384;    // two O tiles of 64
+// P, two tokens to a column, replaces S from its start.
 
 // A lane's own pages.
 constexpr std::uint32_t kSlice = 16;                       // tokens per step
@@ -115,12 +121,13 @@ struct Maps {
     CUtensorMap extent8;
 };
 
-struct Shared {  // behind the ring
+struct Shared {  // behind the ring and the two Q tiles
     std::uint64_t full[kStages];    // K and V landed
     std::uint64_t fixed[kStages];   // V rows of invalid tokens are zero
     std::uint64_t empty[kStages];   // the products are done with the stage
-    std::uint64_t s_full[2];        // S of softmax group w
-    std::uint64_t p_full[2];        // P of softmax group w
+    std::uint64_t s_full[2];        // scores for a softmax group
+    std::uint64_t p_full[kSTiles];  // weights in an S tile
+    std::uint64_t o_done[2];        // the last product into an O tile
     std::uint64_t q_full;
     std::uint64_t o_full;
     std::uint64_t valid[kStages];   // valid tokens of each 8-token group, 4 bits each
@@ -128,7 +135,8 @@ struct Shared {  // behind the ring
     int abort;
 };
 
-constexpr std::size_t kSmemBytes = 1024 + kStages * kStageBytes + sizeof(Shared);
+constexpr std::uint32_t kQBytes = 2 * kTileBytes;
+constexpr std::size_t kSmemBytes = 1024 + kStages * kStageBytes + kQBytes + sizeof(Shared);
 
 __device__ __forceinline__ void report(unsigned int code) { atomicCAS(&g_prefix_status, kErrNone, code); }
 
@@ -166,16 +174,50 @@ __device__ __forceinline__ void tma_load_page(void* dst, CUtensorMap const* map,
         : "memory");
 }
 
+// The products are issued from code that the whole warp runs, each by its one
+// elected lane: descriptors then stay in uniform registers. (Issued inside a
+// branch of one lane, every descriptor is moved there first: 65 clocks per
+// instruction measured, against 32 of work.)
+__device__ __forceinline__ std::uint32_t elect_lane()
+{
+    std::uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e;
+}
+
 // D(tmem) (+)= A(tmem) * B(smem desc).
-__device__ __forceinline__ void mma_ts(std::uint32_t d, std::uint32_t a, std::uint64_t b, std::uint32_t idesc,
-    std::uint32_t accumulate)
+__device__ __forceinline__ void mma_ts(std::uint32_t elected, std::uint32_t d, std::uint32_t a, std::uint64_t b,
+    std::uint32_t idesc, std::uint32_t accumulate)
 {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 q, %0, 0;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%1], [%2], %3, %4, p;\n\t}"
+        ::"r"(elected), "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
+}
+
+// D(tmem) (+)= A(smem desc) * B(smem desc)^T.
+__device__ __forceinline__ void mma_ss(std::uint32_t elected, std::uint32_t d, std::uint64_t a, std::uint64_t b,
+    std::uint32_t idesc, std::uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 q, %0, 0;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%1], %2, %3, %4, p;\n\t}"
+        ::"r"(elected), "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// Arrives on the barrier once the elected lane's products are done.
+__device__ __forceinline__ void commit(std::uint32_t elected, std::uint64_t* bar)
+{
+    if (elected) {
+        tc_commit(bar);
+    }
+    __syncwarp();
 }
 
 // 32 lanes x 32 columns; the caller waits.
@@ -196,19 +238,6 @@ __device__ __forceinline__ void tmem_ld32(std::uint32_t addr, float* v)
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ void tmem_st32(std::uint32_t addr, std::uint32_t const* r)
-{
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0],"
-        " {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22,"
-        " %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
-        ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-          "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
-          "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
-}
-
 __device__ __forceinline__ void tmem_st16(std::uint32_t addr, std::uint32_t const (&r)[16])
 {
     asm volatile(
@@ -224,6 +253,33 @@ __device__ __forceinline__ float exp2_approx(float x)
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// Two FP32 values in one 64-bit register: one instruction for both.
+__device__ __forceinline__ std::uint64_t pack_f32x2(float lo, float hi)
+{
+    std::uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+
+__device__ __forceinline__ void unpack_f32x2(std::uint64_t v, float& lo, float& hi)
+{
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+
+__device__ __forceinline__ std::uint64_t fma_f32x2(std::uint64_t a, std::uint64_t b, std::uint64_t c)
+{
+    std::uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+__device__ __forceinline__ std::uint64_t add_f32x2(std::uint64_t a, std::uint64_t b)
+{
+    std::uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
 
 __device__ __forceinline__ std::uint32_t pack_half2(float lo, float hi)
@@ -242,94 +298,101 @@ __device__ __forceinline__ void produce(Args const& a, Maps const& maps, kk_pref
 {
     std::uint32_t const lane = threadIdx.x % 32u;
     int volatile* abort = &sh->abort;
-    std::uint32_t win = item.desc_begin;
-    std::uint32_t w_slot = 0, w_word = 0, n_slot = 0, n_word = 0;
-    // 32 descriptors at a time, one per lane; the next ones are requested ahead.
-    auto fetch = [&](std::uint32_t at, std::uint32_t& slot, std::uint32_t& word) {
-        std::uint32_t const i = at + lane;
-        slot = word = 0;
-        if (i < item.desc_end) {
-            std::uint32_t const* d = reinterpret_cast<std::uint32_t const*>(a.descs + i);
-            slot = __ldg(d);
-            word = __ldg(d + 2);
-        }
-    };
-    fetch(win, w_slot, w_word);
-    fetch(win + 32u, n_slot, n_word);
-    std::uint32_t e = item.desc_begin;
-    std::uint32_t tile = 0;
     int const block = static_cast<int>(a.layer * 2u);
     int const head = static_cast<int>(item.kv_head);
+    // A window of 32 descriptors from e on, one per lane.
+    std::uint32_t e = item.desc_begin;
+    std::uint32_t slot = 0, tokens = 0, kind = 0;
+    auto fetch = [&]() {
+        std::uint32_t const i = e + lane;
+        slot = tokens = kind = 0;
+        if (i < item.desc_end) {
+            std::uint32_t const* d = reinterpret_cast<std::uint32_t const*>(a.descs + i);
+            std::uint32_t const word = __ldg(d + 2);
+            slot = __ldg(d);
+            tokens = word & 0xffffu;
+            kind = (word >> 16) & 0xffu;
+        }
+    };
+    fetch();
     bool ok = true;
+    std::uint32_t tile = 0;
     for (; tile < item.token_tiles; ++tile) {
         std::uint32_t const s = tile % kStages;
         std::uint32_t const phase = (tile / kStages) & 1u;
         ok = tile < kStages || wait_or_abort(&sh->empty[s], phase ^ 1u, abort);
-        if (!__all_sync(0xffffffffu, ok)) {
-            ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) {
             break;
         }
         std::uint8_t* const k_dst = ring + s * kStageBytes;
         std::uint64_t valid = 0;
-        std::uint32_t n = 0;
-        for (; e < item.desc_end; ++e) {
-            if (e >= win + 32u) {
-                win += 32u;
-                w_slot = n_slot;
-                w_word = n_word;
-                fetch(win + 32u, n_slot, n_word);
-            }
-            std::uint32_t const slot = __shfl_sync(0xffffffffu, w_slot, e - win);
-            std::uint32_t const word = __shfl_sync(0xffffffffu, w_word, e - win);
-            std::uint32_t const tokens = word & 0xffffu;
-            std::uint32_t const kind = (word >> 16) & 0xffu;
+        std::uint32_t n = 0;  // groups of the tile filled
+        for (bool more = true; more;) {
+            // A page outside its pool or over its capacity counts nothing and is reported.
             std::uint32_t const cap = kind == 0 ? a.micro_cap : 64u;
-            if (kind > 1u || slot >= (kind == 0 ? a.micro_slots : a.extent_slots) || tokens > cap) {
-                if (lane == 0) {
-                    report(kErrBadDescriptor);
-                }
-                continue;
+            bool const good = kind <= 1u && slot < (kind == 0 ? a.micro_slots : a.extent_slots) && tokens <= cap;
+            if (!good && e + lane < item.desc_end) {
+                report(kErrBadDescriptor);
             }
-            std::uint32_t const groups = (tokens + 7u) / 8u;
-            if (n + groups > kSlots) {
-                break;
+            std::uint32_t const groups = good ? (tokens + 7u) / 8u : 0u;
+            std::uint32_t last = groups;  // groups of the window up to this lane's
+#pragma unroll
+            for (std::uint32_t o = 1; o < 32u; o *= 2u) {
+                std::uint32_t const x = __shfl_up_sync(0xffffffffu, last, o);
+                last += lane >= o ? x : 0u;
             }
-            bool const whole = groups * 8u == cap;
-            CUtensorMap const* map = kind == 0 ? (whole ? &maps.micro : &maps.micro8)
-                                               : (whole ? &maps.extent : &maps.extent8);
-            std::uint32_t const boxes = whole ? (groups != 0 ? 1u : 0u) : groups;
-            std::uint32_t const box = whole ? groups : 1u;  // groups per box
+            bool const fits = n + last <= kSlots;  // a leading run of the lanes
+            std::uint32_t const taken = __popc(__ballot_sync(0xffffffffu, fits));
+            std::uint32_t const sum = __shfl_sync(0xffffffffu, last, taken == 0 ? 0 : taken - 1u);
+            std::uint32_t const added = taken == 0 ? 0u : sum;
             // Counted before the copies: the phase cannot end before the arrival below.
-            if (lane == 0 && boxes != 0) {
+            if (lane == 0 && added != 0) {
                 asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;"
-                             ::"r"(smem_u32(&sh->full[s])), "r"(2u * groups * 8u * kRowBytes)
+                             ::"r"(smem_u32(&sh->full[s])), "r"(2u * added * 8u * kRowBytes)
                              : "memory");
-                for (std::uint32_t b = 0; b < boxes; ++b) {
-                    std::uint8_t* dst = k_dst + (n + b * box) * 8u * kRowBytes;
-                    tma_load_page(dst, map, &sh->full[s], head, static_cast<int>(b * 8u), block,
+            }
+            __syncwarp();
+            std::uint64_t mine = 0;
+            if (fits && groups != 0) {
+                std::uint32_t const at = n + last - groups;
+                bool const whole = groups * 8u == cap;
+                CUtensorMap const* map = kind == 0 ? (whole ? &maps.micro : &maps.micro8)
+                                                   : (whole ? &maps.extent : &maps.extent8);
+                std::uint32_t const step = whole ? groups : 1u;  // groups per box
+                for (std::uint32_t g = 0; g < groups; g += step) {
+                    std::uint8_t* dst = k_dst + (at + g) * 8u * kRowBytes;
+                    tma_load_page(dst, map, &sh->full[s], head, static_cast<int>(g * 8u), block,
                         static_cast<int>(slot));
-                    tma_load_page(dst + kHalfStage, map, &sh->full[s], head, static_cast<int>(b * 8u), block + 1,
+                    tma_load_page(dst + kTileBytes, map, &sh->full[s], head, static_cast<int>(g * 8u), block + 1,
                         static_cast<int>(slot));
                 }
+                // 8 tokens in every group but the page's last.
+                std::uint64_t const full = groups == 1u ? 0u : kAllValid >> (64u - 4u * (groups - 1u));
+                std::uint64_t const rest = tokens - (groups - 1u) * 8u;
+                mine = (full | (rest << (4u * (groups - 1u)))) << (4u * at);
             }
-            for (std::uint32_t g = 0; g < groups; ++g) {
-                std::uint32_t const left = tokens - g * 8u;
-                valid |= std::uint64_t(left < 8u ? left : 8u) << (4u * (n + g));
-            }
-            n += groups;
+            std::uint32_t const lo = __reduce_or_sync(0xffffffffu, static_cast<std::uint32_t>(mine));
+            std::uint32_t const hi = __reduce_or_sync(0xffffffffu, static_cast<std::uint32_t>(mine >> 32));
+            valid |= (std::uint64_t(hi) << 32) | lo;
+            n += added;
+            e += taken;
+            more = taken == 32u && e < item.desc_end;  // the tile may go on behind the window
+            fetch();
         }
+        e = e < item.desc_end ? e : item.desc_end;
         if (lane == 0) {
             sh->valid[s] = valid;
             mbar_arrive(&sh->full[s]);  // releases valid; the phase ends when the bytes land
         }
         if (valid != kAllValid) {
             ok = wait_or_abort(&sh->full[s], phase, abort);
-            if (!__all_sync(0xffffffffu, ok)) {
-                ok = false;
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) {
                 ++tile;
                 break;
             }
-            std::uint8_t* const v = k_dst + kHalfStage;
+            std::uint8_t* const v = k_dst + kTileBytes;
             for (std::uint32_t i = lane; i < kTile * 8u; i += 32u) {
                 std::uint32_t const t = i / 8u;
                 if (t % 8u >= ((valid >> (4u * (t / 8u))) & 15u)) {
@@ -357,155 +420,133 @@ __device__ __forceinline__ void produce(Args const& a, Maps const& maps, kk_pref
     }
 }
 
-__device__ __forceinline__ void issue(kk_prefix_item const& item, std::uint8_t* ring, Shared* sh)
+// The tiles of an item in turn: turn q works on K/V tile q / 2 for row tile q % 2
+// (two row tiles), or on K/V tile q (one). Its O tile is q % 2, its S tile q % 3.
+__device__ __forceinline__ std::uint32_t turns_of(kk_prefix_item const& item) { return item.token_tiles * item.row_tiles; }
+
+__device__ __forceinline__ void issue(kk_prefix_item const& item, std::uint8_t* ring, std::uint8_t* q_tiles,
+    Shared* sh)
 {
     int volatile* abort = &sh->abort;
+    std::uint32_t const elected = elect_lane();
     std::uint32_t const tmem = sh->tmem;
-    std::uint32_t const n = item.token_tiles;
-    bool const pair = item.row_tiles == 2u;
+    std::uint32_t const turns = turns_of(item);
+    std::uint32_t const pair = item.row_tiles == 2u ? 1u : 0u;
     constexpr std::uint32_t kIdescQK = umma_idesc_f16_f32(128, 128);
     constexpr std::uint32_t kIdescPV = umma_idesc_f16_f32(128, 64) | (1u << 16);  // V is MN-major
-    auto landed = [&](std::uint32_t j) {
-        return wait_or_abort(&sh->full[j % kStages], (j / kStages) & 1u, abort);
+    auto wait = [&](std::uint64_t* bar, std::uint32_t phase) {
+        return __all_sync(0xffffffffu, wait_or_abort(bar, phase & 1u, abort)) != 0;
     };
-    auto qk = [&](std::uint32_t w, std::uint32_t j) {
+    auto scores = [&](std::uint32_t q) {
+        std::uint32_t const j = q >> pair;
+        if (!wait(&sh->full[j % kStages], j / kStages)) {
+            return false;
+        }
+        std::uint64_t const q_desc = umma_desc_k_sw128(q_tiles + (q & pair) * kTileBytes);
         std::uint64_t const k_desc = umma_desc_k_sw128(ring + (j % kStages) * kStageBytes);
 #pragma unroll
         for (std::uint32_t k = 0; k < kHeadDim / 16u; ++k) {
-            mma_ts(tmem + kColS + w * kTile, tmem + kColQ + w * 32u + k * 8u, k_desc + k * 2u, kIdescQK, k != 0);
+            mma_ss(elected, tmem + kColS + (q % kSTiles) * kTile, q_desc + k * 2u, k_desc + k * 2u, kIdescQK, k != 0);
         }
-        tc_commit(&sh->s_full[w]);
+        commit(elected, &sh->s_full[q % 2u]);
+        return true;
     };
-    // P V of a group: FP16 high halves, then the low halves.
-    auto pv = [&](std::uint32_t w, std::uint32_t j, bool first) {
-        std::uint64_t const v_desc = umma_desc_k_sw128(ring + (j % kStages) * kStageBytes + kHalfStage);
-        std::uint32_t const p = tmem + kColS + w * kTile;
-        std::uint32_t const o = tmem + kColO + w * kHeadDim;
-#pragma unroll
-        for (std::uint32_t k = 0; k < kTile / 16u; ++k) {
-            std::uint64_t const b = v_desc + k * (16u * kRowBytes / 16u);
-            mma_ts(o, p + k * 8u, b, kIdescPV, !(first && k == 0));
-            mma_ts(o, p + kColPLo + k * 8u, b, kIdescPV, 1u);
-        }
-    };
-    auto weights = [&](std::uint32_t w, std::uint32_t k, std::uint32_t j) {  // the group's k-th P, on tile j
-        bool const ok = wait_or_abort(&sh->fixed[j % kStages], (j / kStages) & 1u, abort)
-            && wait_or_abort(&sh->p_full[w], k & 1u, abort);
-        tc_fence_after();
-        return ok;
-    };
-    bool ok = wait_or_abort(&sh->q_full, 0, abort) && landed(0);
+    bool ok = wait(&sh->q_full, 0);
     tc_fence_after();
-    if (ok) {
-        qk(0, 0);
-        if (pair) {
-            qk(1, 0);
-        } else if (n > 1u) {
-            ok = landed(1);
-            if (ok) {
-                qk(1, 1);
-            }
+    for (std::uint32_t q = 0; ok && q < kSTiles && q < turns; ++q) {
+        ok = scores(q);
+    }
+    for (std::uint32_t q = 0; ok && q < turns; ++q) {
+        std::uint32_t const j = q >> pair;
+        ok = wait(&sh->fixed[j % kStages], j / kStages) && wait(&sh->p_full[q % kSTiles], q / kSTiles);
+        if (!ok) {
+            break;
+        }
+        tc_fence_after();
+        std::uint64_t const v_desc = umma_desc_k_sw128(ring + (j % kStages) * kStageBytes + kTileBytes);
+        std::uint32_t const o = tmem + kColO + (q % 2u) * kHeadDim;
+#pragma unroll
+        for (std::uint32_t i = 0; i < kTile / 16u; ++i) {
+            std::uint32_t const p = tmem + kColS + (q % kSTiles) * kTile + i * 8u;
+            std::uint64_t const b = v_desc + i * 16u * (kRowBytes / 16u);
+            mma_ts(elected, o, p, b, kIdescPV, q >= 2u || i != 0);
+        }
+        commit(elected, &sh->o_done[q % 2u]);
+        if (!pair || q % 2u == 1u) {
+            commit(elected, &sh->empty[j % kStages]);
+        }
+        // The scores that overwrite these weights are issued behind the
+        // product that reads them; the tensor core runs the two in that order.
+        if (q + kSTiles < turns) {
+            ok = scores(q + kSTiles);
         }
     }
-    // The product that overwrites S of a group is issued behind the one that
-    // reads P from the same columns; the tensor core runs them in that order.
-    for (std::uint32_t j = 0; ok && j < n; ++j) {
-        if (pair) {
-            for (std::uint32_t w = 0; w < 2u && ok; ++w) {
-                ok = weights(w, j, j);
-                if (!ok) {
-                    break;
-                }
-                pv(w, j, j == 0);
-                if (w == 1u) {
-                    tc_commit(&sh->empty[j % kStages]);
-                }
-                if (j + 1u < n) {
-                    ok = landed(j + 1u);
-                    if (ok) {
-                        qk(w, j + 1u);
-                    }
-                }
-            }
-        } else {
-            std::uint32_t const w = j & 1u;
-            ok = weights(w, j >> 1, j);
-            if (!ok) {
-                break;
-            }
-            pv(w, j, j < 2u);
-            tc_commit(&sh->empty[j % kStages]);
-            if (j + 2u < n) {
-                ok = landed(j + 2u);
-                if (ok) {
-                    qk(w, j + 2u);
-                }
-            }
-        }
-    }
-    tc_commit(&sh->o_full);
+    commit(elected, &sh->o_full);
     if (!ok) {
         mbar_wait(&sh->o_full, 0, nullptr);  // no product outlives the TMEM
     }
 }
 
-// One thread per query row: warp % 4 selects the TMEM lanes, warp / 4 the group.
-__device__ __forceinline__ void soften(Args const& a, kk_prefix_item const& item, kk_prefix_group const& g,
-    std::uint8_t* ring, Shared* sh)
+// One thread per query row: warp % 4 selects the TMEM lanes, warp / 4 the group,
+// which serves every second turn.
+__device__ __forceinline__ void soften(Args const& a, kk_prefix_item const& item, std::uint8_t* ring,
+    std::uint8_t* q_tiles, Shared* sh)
 {
     int volatile* abort = &sh->abort;
     std::uint32_t const warp = threadIdx.x / 32u;
     std::uint32_t const lane = threadIdx.x % 32u;
-    std::uint32_t const w = warp / 4u;
-    bool const pair = item.row_tiles == 2u;
+    std::uint32_t const t = warp / 4u;  // group and O tile
+    std::uint32_t const pair = item.row_tiles == 2u ? 1u : 0u;
     std::uint32_t const r = (warp % 4u) * 32u + lane;
-    std::uint32_t const tile_row = (item.row_tile + (pair ? w : 0u)) * kTile;
-    std::uint32_t const rows = g.lane_count * a.group;
+    std::uint32_t const tile_row = (item.row_tile + (t & pair)) * kTile;
+    std::uint32_t const rows = item.lane_count * a.group;
     bool const mine = tile_row + r < rows;
     bool const any = tile_row + (warp % 4u) * 32u < rows;  // some row of this warp exists
     std::uint32_t const tmem = sh->tmem + ((warp % 4u) * 32u << 16);
-    std::uint32_t const s_col = tmem + kColS + w * kTile;
-    std::uint32_t const o_col = tmem + kColO + w * kHeadDim;
+    std::uint32_t const o_col = tmem + kColO + t * kHeadDim;
 
-    {
-        std::uint32_t q[32];
+    if (pair || t == 0) {
+        uint4 q[8];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            q[i] = 0;
+        for (int i = 0; i < 8; ++i) {
+            q[i] = make_uint4(0, 0, 0, 0);
         }
         if (mine) {
             std::uint32_t const row = tile_row + r;
-            std::uint32_t const query_row = a.lanes[g.lane_begin + row / a.group].query_row;
+            std::uint32_t const query_row = a.lanes[item.lane_begin + row / a.group].query_row;
             uint4 const* src = reinterpret_cast<uint4 const*>(a.query + query_row * a.query_stride
                 + (item.kv_head * a.group + row % a.group) * kHeadDim);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                uint4 const x = src[i];
-                q[4 * i] = x.x;
-                q[4 * i + 1] = x.y;
-                q[4 * i + 2] = x.z;
-                q[4 * i + 3] = x.w;
+                q[i] = src[i];
             }
         }
-        tmem_st32(tmem + kColQ + w * 32u, q);
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-            mbar_arrive(&sh->q_full);
+        std::uint8_t* const dst = q_tiles + t * kTileBytes + r * kRowBytes;
+#pragma unroll
+        for (std::uint32_t i = 0; i < 8u; ++i) {
+            *reinterpret_cast<uint4*>(dst + ((i ^ (r & 7u)) << 4)) = q[i];
         }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncwarp();
+    if (lane == 0) {
+        mbar_arrive(&sh->q_full);
     }
 
+    auto wait = [&](std::uint64_t* bar, std::uint32_t phase) {
+        return __all_sync(0xffffffffu, wait_or_abort(bar, phase & 1u, abort)) != 0;
+    };
+    std::uint32_t const turns = turns_of(item);
     float m = -INFINITY;  // reference maximum of the row, log2 units
     float l = 0.f;
-    std::uint32_t k = 0;
     bool ok = true;
-    for (std::uint32_t j = pair ? 0u : w; j < item.token_tiles; j += pair ? 1u : 2u, ++k) {
-        std::uint32_t const s = j % kStages;
-        ok = wait_or_abort(&sh->full[s], (j / kStages) & 1u, abort)
-            && wait_or_abort(&sh->s_full[w], k & 1u, abort);
-        if (!__all_sync(0xffffffffu, ok)) {
-            ok = false;
+    for (std::uint32_t q = t; q < turns; q += 2u) {
+        std::uint32_t const k = q / 2u;  // turn of this group
+        std::uint32_t const j = q >> pair;
+        std::uint32_t const buf = q % kSTiles;
+        std::uint32_t const s_col = tmem + kColS + buf * kTile;
+        ok = wait(&sh->s_full[t], k) && wait(&sh->full[j % kStages], j / kStages);
+        if (!ok) {
             break;
         }
         tc_fence_after();
@@ -515,7 +556,7 @@ __device__ __forceinline__ void soften(Args const& a, kk_prefix_item const& item
             for (std::uint32_t c = 0; c < 4u; ++c) {
                 tmem_ld32(s_col + c * 32u, x + c * 32u);
             }
-            std::uint64_t const valid = sh->valid[s];
+            std::uint64_t const valid = sh->valid[j % kStages];
             tmem_wait_ld();
             if (valid != kAllValid) {
 #pragma unroll
@@ -523,110 +564,124 @@ __device__ __forceinline__ void soften(Args const& a, kk_prefix_item const& item
                     x[i] = (i % 8u) < (static_cast<std::uint32_t>(valid >> (4u * (i / 8u))) & 15u) ? x[i] : -INFINITY;
                 }
             }
-            float top[4] = {x[0], x[1], x[2], x[3]};
+            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (std::uint32_t i = 4; i < kTile; ++i) {
-                top[i % 4u] = fmaxf(top[i % 4u], x[i]);
+            for (std::uint32_t i = 0; i < kTile; i += 2u) {
+                top[i / 2u % 4u] = fmaxf(fmaxf(top[i / 2u % 4u], x[i]), x[i + 1u]);
             }
             float const mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
             bool const grow = mt > m + kRescale || m == -INFINITY;
             if (__any_sync(0xffffffffu, grow)) {
-                float const m_new = grow ? mt : m;
-                float const alpha = m == -INFINITY || !grow ? 1.f : exp2_approx(m - m_new);
-                m = m_new;
+                float const now = grow ? mt : m;
+                float const alpha = m == -INFINITY ? 1.f : exp2_approx(m - now);
+                m = now;
                 l *= alpha;
                 if (k != 0) {
-                    // S of this tile was issued behind the previous P V, so O is at rest.
+                    // Once the last product into O is done.
+                    ok = wait(&sh->o_done[t], k - 1u);
+                    if (!ok) {
+                        break;
+                    }
+                    tc_fence_after();
+#pragma unroll 1
+                    for (std::uint32_t c = 0; c < kHeadDim / 16u; ++c) {
+                        float o[16];
+                        tmem_ld16(o_col + c * 16u, o);
 #pragma unroll
-                    for (std::uint32_t c = 0; c < 2u; ++c) {
-                        float o[32];
-                        tmem_ld32(o_col + c * 32u, o);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) {
+                        for (int i = 0; i < 16; ++i) {
                             o[i] *= alpha;
                         }
-                        tmem_st32(o_col + c * 32u, reinterpret_cast<std::uint32_t const*>(o));
+                        tmem_st16(o_col + c * 16u, reinterpret_cast<std::uint32_t const(&)[16]>(o));
                     }
                 }
             }
-            float const m_use = m == -INFINITY ? 0.f : m;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            float const shift = m == -INFINITY ? 0.f : -m;
+            std::uint64_t const scale2 = pack_f32x2(a.scale_log2, a.scale_log2);
+            std::uint64_t const shift2 = pack_f32x2(shift, shift);
+            std::uint64_t sum2[2] = {0, 0};
 #pragma unroll
             for (std::uint32_t c = 0; c < 4u; ++c) {
-                std::uint32_t hi[16], lo[16];
+                std::uint32_t p[16];
 #pragma unroll
                 for (std::uint32_t i = 0; i < 16u; ++i) {
-                    float const p0 = exp2_approx(fmaf(x[c * 32u + 2u * i], a.scale_log2, -m_use));
-                    float const p1 = exp2_approx(fmaf(x[c * 32u + 2u * i + 1u], a.scale_log2, -m_use));
-                    sum[(2u * i) % 4u] += p0;
-                    sum[(2u * i + 1u) % 4u] += p1;
-                    float const h0 = leading(p0), h1 = leading(p1);
-                    hi[i] = pack_half2(h0, h1);
-                    lo[i] = pack_half2(p0 - h0, p1 - h1);
+                    std::uint32_t const at = c * 32u + 2u * i;
+                    float p0, p1;
+                    unpack_f32x2(fma_f32x2(pack_f32x2(x[at], x[at + 1u]), scale2, shift2), p0, p1);
+                    p0 = exp2_approx(p0);
+                    p1 = exp2_approx(p1);
+                    sum2[i % 2u] = add_f32x2(sum2[i % 2u], pack_f32x2(p0, p1));
+                    p[i] = pack_half2(p0, p1);
                 }
-                tmem_st16(s_col + c * 16u, hi);
-                tmem_st16(s_col + kColPLo + c * 16u, lo);
+                tmem_st16(s_col + c * 16u, p);
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            float s0, s1;
+            unpack_f32x2(add_f32x2(sum2[0], sum2[1]), s0, s1);
+            l += s0 + s1;
             tmem_wait_st();
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-            mbar_arrive(&sh->p_full[w]);
+            mbar_arrive(&sh->p_full[buf]);
         }
     }
-    ok = ok && wait_or_abort(&sh->o_full, 0, abort);
-    ok = __all_sync(0xffffffffu, ok);
+    ok = ok && wait(&sh->o_full, 0);
     tc_fence_after();
-    float o[kHeadDim];
-    if (ok && any && k != 0) {
-        tmem_ld32(o_col, o);
-        tmem_ld32(o_col + 32u, o + 32);
-        tmem_wait_ld();
-    } else {
-#pragma unroll
-        for (std::uint32_t i = 0; i < kHeadDim; ++i) {
-            o[i] = 0.f;
-        }
-    }
-    // One row tile: the second group's half of the tokens joins the first's
-    // through the ring, which nothing uses any more.
+    // One row tile: the second group's O joins the first's through the ring,
+    // which nothing uses any more.
     constexpr std::uint32_t kStride = kHeadDim + 3;  // odd: rows fall into different banks
-    float* const join = reinterpret_cast<float*>(ring) + r * kStride;
-    if (!pair && w == 1u && ok) {
+    static_assert(kTile * kStride * 4 <= kStages * kStageBytes, "room for one O tile");
+    float* const other = reinterpret_cast<float*>(ring) + r * kStride;
+    if (!pair && t == 1u && ok) {
+        bool const holds = any && turns > 1u;
 #pragma unroll
-        for (std::uint32_t i = 0; i < kHeadDim; ++i) {
-            join[i] = o[i];
+        for (std::uint32_t c = 0; c < 4u; ++c) {
+            float o[16];
+            if (holds) {
+                tmem_ld16(o_col + c * 16u, o);
+            }
+#pragma unroll
+            for (std::uint32_t i = 0; i < 16u; ++i) {
+                other[c * 16u + i] = holds ? o[i] : 0.f;
+            }
         }
-        join[kHeadDim] = m;
-        join[kHeadDim + 1] = l;
+        other[kHeadDim] = m;
+        other[kHeadDim + 1] = l;
     }
     asm volatile("bar.sync 1, 256;" ::: "memory");  // the 8 softmax warps, all of which come here
-    if (!pair && (w == 1u || !ok)) {
+    if ((!pair && t == 1u) || !ok || !any) {
         return;
     }
+    float f0 = 1.f, f1 = 0.f;
     if (!pair) {
-        float const m1 = join[kHeadDim];
+        float const m1 = other[kHeadDim];
         float const top = fmaxf(m, m1);
         float const use = top == -INFINITY ? 0.f : top;
-        float const f0 = exp2_approx(m - use), f1 = exp2_approx(m1 - use);
+        f0 = exp2_approx(m - use);
+        f1 = exp2_approx(m1 - use);
         m = top;
-        l = l * f0 + join[kHeadDim + 1] * f1;
+        l = l * f0 + other[kHeadDim + 1] * f1;
+    }
+    std::uint64_t const row = std::uint64_t(item.part_row) + (t & pair) * kTile + r;
+    float4* const dst = reinterpret_cast<float4*>(a.part_o + row * kHeadDim);
 #pragma unroll
-        for (std::uint32_t i = 0; i < kHeadDim; ++i) {
-            o[i] = o[i] * f0 + join[i] * f1;
+    for (std::uint32_t c = 0; c < 4u; ++c) {
+        float o[16];
+        tmem_ld16(o_col + c * 16u, o);  // the whole warp, also for rows that do not exist
+        if (!pair) {
+#pragma unroll
+            for (std::uint32_t i = 0; i < 16u; ++i) {
+                o[i] = o[i] * f0 + other[c * 16u + i] * f1;
+            }
+        }
+        if (mine) {
+#pragma unroll
+            for (std::uint32_t i = 0; i < 4u; ++i) {
+                dst[c * 4u + i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            }
         }
     }
-    if (mine && ok) {
-        std::uint64_t const row = g.part_row
-            + (std::uint64_t(item.kv_head * g.part_count + item.part) * g.row_tiles) * kTile + tile_row + r;
-        float4* dst = reinterpret_cast<float4*>(a.part_o + row * kHeadDim);
-#pragma unroll
-        for (std::uint32_t i = 0; i < kHeadDim / 4u; ++i) {
-            dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-        }
+    if (mine) {
         a.part_ml[row] = make_float2(m, l);
     }
 }
@@ -677,19 +732,11 @@ __device__ __forceinline__ void own_task(Args const& a, kk_prefix_item const& it
     std::uint32_t const mi = lane >> 3;
     std::uint32_t const r8 = lane & 7u;
     std::uint32_t const G = a.group;
-    kk_attn_lane const ln = a.lanes[item.owner];
-    std::uint64_t const row0 = std::uint64_t(ln.item_offset) + std::uint64_t(item.part) * a.plan.q_heads
-        + item.kv_head * G;
-    if (item.part >= ln.item_count || row0 + G > a.plan.part_rows) {
-        if (lane == 0) {
-            report(kErrBadArgument);
-        }
-        return;
-    }
+    std::uint64_t const row0 = item.part_row;
     // Queries as B fragments of S^T = K Q^T; heads past the group are zero.
     std::uint32_t qf[NT][4][2];
     {
-        __half const* q = a.query + ln.query_row * a.query_stride + item.kv_head * G * kHeadDim;
+        __half const* q = a.query + item.query_row * a.query_stride + item.kv_head * G * kHeadDim;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             std::uint32_t const h = nt * 8u + g;
@@ -905,11 +952,12 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_attention_kernel(const __g
     extern __shared__ std::uint8_t smem_raw[];
     std::uint32_t const pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;  // swizzle atoms are 1 KB
     std::uint8_t* const ring = smem_raw + pad;
-    Shared* const sh = reinterpret_cast<Shared*>(ring + kStages * kStageBytes);
+    std::uint8_t* const q_tiles = ring + kStages * kStageBytes;
+    Shared* const sh = reinterpret_cast<Shared*>(q_tiles + kQBytes);
     std::uint32_t const warp = threadIdx.x / 32u;
-    pdl_launch_dependents();
     if (blockIdx.x >= a.plan.num_shared) {
         pdl_wait();
+        pdl_launch_dependents();  // behind the wait: the joining launch reads the plan before its own
         if (warp >= kSoftWarps) {
             return;
         }
@@ -920,7 +968,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_attention_kernel(const __g
         for (std::uint32_t t = warp; t < count; t += kSoftWarps) {
             kk_prefix_item const item = a.items[a.plan.num_shared + first + t];
             if (item.row_tiles != 0 || item.owner >= a.plan.num_lanes || item.kv_head >= a.kv_heads
-                || item.desc_begin > item.desc_end || item.desc_end > a.plan.num_descs) {
+                || item.desc_begin > item.desc_end || item.desc_end > a.plan.num_descs
+                || std::uint64_t(item.part_row) + a.group > a.plan.part_rows) {
                 if (threadIdx.x % 32u == 0) {
                     report(kErrBadArgument);
                 }
@@ -936,53 +985,53 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_attention_kernel(const __g
             mbar_init(&sh->fixed[s], 1);
             mbar_init(&sh->empty[s], 1);
         }
-        for (int w = 0; w < 2; ++w) {
-            mbar_init(&sh->s_full[w], 1);
-            mbar_init(&sh->p_full[w], 4);
+        for (std::uint32_t i = 0; i < kSTiles; ++i) {
+            mbar_init(&sh->p_full[i], 4);
         }
+        mbar_init(&sh->s_full[0], 1);
+        mbar_init(&sh->s_full[1], 1);
+        mbar_init(&sh->o_done[0], 1);
+        mbar_init(&sh->o_done[1], 1);
         mbar_init(&sh->q_full, kSoftWarps);
         mbar_init(&sh->o_full, 1);
         sh->abort = 0;
         fence_barrier_init();
-    }
-    pdl_wait();
-    kk_prefix_item const item = a.items[blockIdx.x];
-    kk_prefix_group g{};
-    bool fits = item.owner < a.plan.num_groups;
-    if (fits) {
-        g = a.groups[item.owner];
-        fits = (item.row_tiles == 1u || item.row_tiles == 2u) && item.kv_head < a.kv_heads
-            && item.desc_begin <= item.desc_end && item.desc_end <= a.plan.num_descs && item.token_tiles != 0
-            && item.row_tile + item.row_tiles <= g.row_tiles && item.part < g.part_count
-            && g.lane_begin <= a.plan.num_lanes && g.lane_count <= a.plan.num_lanes - g.lane_begin
-            && std::uint64_t(g.part_row) + std::uint64_t(a.kv_heads) * g.part_count * g.row_tiles * kTile
-                <= a.plan.part_rows;
-    }
-    if (!fits) {  // the same for every thread
-        if (threadIdx.x == 0) {
-            report(kErrBadArgument);
-        }
-        return;
     }
     if (warp == kIssuerWarp) {
         tmem_alloc(&sh->tmem, kTmemCols);
         tmem_relinquish();
         tc_fence_before();
     }
+    if (warp == kProducerWarp && threadIdx.x % 32u < 4u) {
+        CUtensorMap const* const all[4] = {&maps.micro, &maps.micro8, &maps.extent, &maps.extent8};
+        prefetch_tensormap(all[threadIdx.x % 4u]);
+    }
+    pdl_wait();
+    pdl_launch_dependents();
+    kk_prefix_item const item = a.items[blockIdx.x];
+    // The same for every thread.
+    bool const fits = (item.row_tiles == 1u || item.row_tiles == 2u) && item.kv_head < a.kv_heads
+        && item.desc_begin <= item.desc_end && item.desc_end <= a.plan.num_descs && item.token_tiles != 0
+        && item.owner < a.plan.num_groups && item.lane_begin <= a.plan.num_lanes
+        && item.lane_count <= a.plan.num_lanes - item.lane_begin
+        && (item.row_tile + item.row_tiles - 1u) * kTile < std::uint64_t(item.lane_count) * a.group
+        && std::uint64_t(item.part_row) + item.row_tiles * kTile <= a.plan.part_rows;
+    if (!fits && threadIdx.x == 0) {
+        report(kErrBadArgument);
+    }
     __syncthreads();
     tc_fence_after();
-    if (warp < kSoftWarps) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
-        soften(a, item, g, ring, sh);
-    } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
-        if (warp == kProducerWarp) {
-            produce(a, maps, item, ring, sh);
-        } else if (warp == kIssuerWarp) {
-            if (threadIdx.x % 32u == 0) {
-                issue(item, ring, sh);
+    if (fits) {
+        if (warp < kSoftWarps) {
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
+            soften(a, item, ring, q_tiles, sh);
+        } else {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
+            if (warp == kProducerWarp) {
+                produce(a, maps, item, ring, sh);
+            } else if (warp == kIssuerWarp) {
+                issue(item, ring, q_tiles, sh);
             }
-            __syncwarp();
         }
     }
     tc_fence_before();
@@ -1002,14 +1051,14 @@ constexpr std::uint32_t kJoinBatch = 8;  // partials requested at once
 // 2^(m_i - m) l_i over the row's partials, in their order.
 __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(const __grid_constant__ Args a)
 {
-    pdl_launch_dependents();
-    pdl_wait();
     std::uint32_t const t = blockIdx.x * kJoinThreads + threadIdx.x;
     std::uint32_t const q_heads = a.plan.q_heads;
     std::uint32_t const lane = t / 16u / q_heads;
     if (lane >= a.plan.num_lanes) {
         return;
     }
+    // The plan is older than the launch that writes the partials: it is read
+    // before that one has ended.
     std::uint32_t const qh = t / 16u % q_heads;
     std::uint32_t const d0 = t % 16u * 4u;
     kk_attn_lane const ln = a.lanes[lane];
@@ -1029,6 +1078,8 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(const __grid_
         report(kErrBadArgument);
         return;
     }
+    pdl_launch_dependents();
+    pdl_wait();
     float m = -INFINITY, l = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     for (std::uint32_t i0 = 0; i0 < count; i0 += kJoinBatch) {
@@ -1264,7 +1315,8 @@ int kk_prefix_attention_plan(const kk_page_desc* descs, uint32_t num_descs, kk_a
             for (std::uint32_t h = 0; h < kv_heads; ++h) {
                 for (std::uint32_t r = 0; r < g.row_tiles; r += 2u) {
                     put(kk_prefix_item{i, h, begin, end, part, static_cast<std::uint16_t>(r),
-                        static_cast<std::uint16_t>(g.row_tiles - r > 1u ? 2u : 1u), closed - before, 0});
+                        static_cast<std::uint16_t>(g.row_tiles - r > 1u ? 2u : 1u), closed - before,
+                        g.part_row + ((h * parts + part) * g.row_tiles + r) * kTile, g.lane_begin, g.lane_count, 0, 0});
                 }
             }
             ++part;
@@ -1307,7 +1359,8 @@ int kk_prefix_attention_plan(const kk_page_desc* descs, uint32_t num_descs, kk_a
                 held += 8u * groupsOf(descs[e]);
                 if (held >= goal || e + 1u == end) {
                     for (std::uint32_t h = 0; h < kv_heads; ++h) {
-                        put(kk_prefix_item{b, h, begin, e + 1u, ln.item_count, 0, 0, 0, 0});
+                        put(kk_prefix_item{b, h, begin, e + 1u, ln.item_count, 0, 0, 0,
+                            static_cast<std::uint32_t>(part_rows) + h * ratio, 0, 0, ln.query_row, 0});
                     }
                     ++ln.item_count;
                     part_rows += q_heads;

@@ -147,6 +147,9 @@ def test_plan_covers_every_page_once(kk, seed, sms):
                 tiles = min(2, grp.row_tiles - at)
                 run = shared.pop((g, h, at, tiles))
                 assert [r.part for r in run] == list(range(grp.part_count))
+                assert [r.part_row for r in run] == [grp.part_row + ((h * grp.part_count + i) * grp.row_tiles + at) * 128
+                                                     for i in range(grp.part_count)]
+                assert all((r.lane_begin, r.lane_count) == (grp.lane_begin, grp.lane_count) for r in run)
                 edges = [r.desc_begin for r in run] + [run[-1].desc_end]
                 assert edges[0] == grp.desc_offset and edges[-1] == grp.desc_offset + grp.desc_count
                 assert all(r.desc_end == e for r, e in zip(run, edges[1:]))
@@ -166,6 +169,7 @@ def test_plan_covers_every_page_once(kk, seed, sms):
         for h in range(hkv):
             run = own.pop((b, h), [])
             assert [r.part for r in run] == list(range(ln.item_count))
+            assert [r.part_row for r in run] == [ln.item_offset + i * hq + h * G for i in range(ln.item_count)]
             if run:
                 edges = [r.desc_begin for r in run] + [run[-1].desc_end]
                 assert edges[0] == ln.desc_offset and edges[-1] == ln.desc_offset + ln.desc_count
@@ -520,9 +524,9 @@ def test_prefix_reports_bad_pages_and_items(kk):
     s.desc.descs = p(s.dev[0])
     # Items that do not fit the plan are reported and write nothing outside the workspace.
     n = s.plan.num_items
-    for at, change in ((0, dict(owner=9)), (0, dict(kv_head=2)), (0, dict(desc_end=nd + 1)), (0, dict(part=99)),
+    for at, change in ((0, dict(owner=9)), (0, dict(kv_head=2)), (0, dict(desc_end=nd + 1)), (0, dict(part_row=(1 << 32) - 1)),
                        (0, dict(row_tile=5)), (0, dict(row_tiles=3)), (0, dict(token_tiles=0)), (n - 1, dict(owner=2)),
-                       (n - 1, dict(part=9)), (n - 1, dict(desc_begin=nd, desc_end=nd - 1)), (n - 1, dict(row_tiles=1))):
+                       (0, dict(lane_count=3)), (0, dict(lane_begin=1 << 31)), (n - 1, dict(part_row=s.plan.part_rows - 3)), (n - 1, dict(desc_begin=nd, desc_end=nd - 1)), (n - 1, dict(row_tiles=1))):
         items = (kk.PrefixItem * n)(*s.items[:n])
         for name, value in change.items():
             setattr(items[at], name, value)
