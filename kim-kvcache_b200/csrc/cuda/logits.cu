@@ -5,11 +5,11 @@
 // 256 tokens at a time (text names low ids far more often than high ones:
 // with one contiguous slice per CTA the first one had half of the history). A CTA
 //  1. counts, in shared memory, what of the row's history is its own (every CTA
-//     reads the whole history) and lists each token at its first occurrence;
-//  2. replaces the counts of the listed tokens by their penalised logits;
+//     reads the whole history) and marks the tokens, a bit each;
+//  2. lists the marked tokens and replaces their counts by their penalised logits;
 //  3. adds the biases to those, or to the plain logits;
-//  4. streams its logits, 16 bytes a thread at a time (rows that start on odd
-//     addresses included), takes the replaced ones from shared memory, applies
+//  4. streams its logits, 256 tokens a warp at a time (rows that start on odd
+//     addresses included), takes the marked ones from shared memory, applies
 //     the mask and keeps the highest; the cluster's winners meet in its first
 //     CTA.
 // Few tokens of a vocabulary are ever penalised, but few warps of the stream
@@ -19,7 +19,7 @@
 // HBM bounds it: 4 bytes read and 4 written per logit. The CTA's logits are
 // asked into L2 at the start, so that DRAM works while the history is counted.
 // Measured on 256 rows of 128,000 logits with about 10,000 tokens of history
-// each (262 MB, 40 us at the measured copy rate): @@LARGE@@; 132 us
+// each (262 MB, 40 us at the measured copy rate): 130 us; 132 us
 // with the penalties inside the stream (82 instructions a logit); 150 us with
 // contiguous slices and a second pass over the history in place of the list;
 // 200 us with each history read once and counted through distributed shared
@@ -36,13 +36,13 @@ __device__ unsigned int g_logits_status;
 
 namespace {
 
-constexpr std::uint32_t kThreads = 384;
+constexpr std::uint32_t kThreads = 256;
+constexpr std::uint32_t kWarps = kThreads / 32;
 constexpr std::uint32_t kMaxCluster = 8;
 constexpr std::uint32_t kBlock = 256;          // consecutive tokens of one CTA
-constexpr std::uint32_t kVecs = 2;             // 16-byte loads in flight per thread
-constexpr std::uint32_t kQuads = 4;            // 16-byte history loads in flight per thread
-constexpr std::uint32_t kPrompt = 0x80000000u; // the prompt names the token; below: occurrences in the output
-constexpr std::uint32_t kListed = 2048;        // tokens listed at most; with more, step 2 looks at every word
+constexpr std::uint32_t kQuads = 2;            // 16-byte history loads in flight per thread
+constexpr std::uint32_t kListed = 2048;        // marked tokens listed at most; others are taken bit by bit
+constexpr std::uint32_t kGather = 2;           // listed tokens per thread at a time
 constexpr std::uint32_t kMaxSharedBytes = 222u * 1024u;
 
 struct LogitsArgs {
@@ -74,6 +74,14 @@ __device__ __forceinline__ void st_cluster_u64(std::uint32_t addr, std::uint64_t
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
 }
 
+// A read-only load issued where it stands in the program.
+__device__ __forceinline__ std::uint32_t ldg_u32_now(void const* p)
+{
+    std::uint32_t v;
+    asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+
 // A logit and its token as one key: a higher logit wins, then a lower id; 0 is
 // below every candidate. NaN and -inf give 0.
 __device__ __forceinline__ std::uint64_t candidate(float x, std::uint32_t id)
@@ -86,10 +94,10 @@ __device__ __forceinline__ std::uint64_t candidate(float x, std::uint32_t id)
     return (std::uint64_t(order) << 32) | (0xffffffffu - id);
 }
 
-__global__ void __launch_bounds__(kThreads, 3) logits_process_kernel(const __grid_constant__ LogitsArgs a)
+__global__ void __launch_bounds__(kThreads, 4) logits_process_kernel(const __grid_constant__ LogitsArgs a)
 {
     extern __shared__ __align__(16) std::uint32_t s_words[];
-    __shared__ std::uint64_t s_best[kThreads / 32];
+    __shared__ std::uint64_t s_best[kWarps];
     __shared__ std::uint64_t s_cluster[kMaxCluster];
     __shared__ std::uint32_t s_listed;
     pdl_launch_dependents();
@@ -123,7 +131,24 @@ __global__ void __launch_bounds__(kThreads, 3) logits_process_kernel(const __gri
     };
     auto in_head = [&](std::uint32_t v) { return v < head && rank == 0; };
 
-    // ---- everything that can be asked for at once: logits, the row's lists
+    // ---- everything that can be asked for at once
+    float rep = 1.f, pres = 0.f, freq = 0.f;
+    std::uint32_t h0 = 0, h1 = 0, prompt = 0, b0 = 0, b1 = 0, mask_row = row;
+    if (d.history_offsets != nullptr) {
+        h0 = ldg_u32_now(d.history_offsets + row);
+        h1 = ldg_u32_now(d.history_offsets + row + 1);
+        rep = d.repetition != nullptr ? __uint_as_float(ldg_u32_now(d.repetition + row)) : 1.f;
+        pres = d.presence != nullptr ? __uint_as_float(ldg_u32_now(d.presence + row)) : 0.f;
+        freq = d.frequency != nullptr ? __uint_as_float(ldg_u32_now(d.frequency + row)) : 0.f;
+        prompt = d.prompt_counts != nullptr ? ldg_u32_now(d.prompt_counts + row) : 0u;
+    }
+    if (d.bias_offsets != nullptr) {
+        b0 = ldg_u32_now(d.bias_offsets + row);
+        b1 = ldg_u32_now(d.bias_offsets + row + 1);
+    }
+    if (d.mask != nullptr && d.mask_rows != nullptr) {
+        mask_row = ldg_u32_now(d.mask_rows + row);
+    }
     for (std::uint32_t i = tid; i < blocks; i += kThreads) {
         std::uint32_t const v = token_of(i * kBlock);
         std::uint32_t const n = (vocab - v < kBlock ? vocab - v : kBlock) / 4u;
@@ -144,23 +169,6 @@ __global__ void __launch_bounds__(kThreads, 3) logits_process_kernel(const __gri
         if (tid == 0) {
             s_listed = 0;
         }
-    }
-    float rep = 1.f, pres = 0.f, freq = 0.f;
-    std::uint32_t h0 = 0, h1 = 0, prompt = 0, b0 = 0, b1 = 0, mask_row = row;
-    if (d.history_offsets != nullptr) {
-        h0 = d.history_offsets[row];
-        h1 = d.history_offsets[row + 1];
-        rep = d.repetition != nullptr ? d.repetition[row] : 1.f;
-        pres = d.presence != nullptr ? d.presence[row] : 0.f;
-        freq = d.frequency != nullptr ? d.frequency[row] : 0.f;
-        prompt = d.prompt_counts != nullptr ? d.prompt_counts[row] : 0u;
-    }
-    if (d.bias_offsets != nullptr) {
-        b0 = d.bias_offsets[row];
-        b1 = d.bias_offsets[row + 1];
-    }
-    if (d.mask != nullptr && d.mask_rows != nullptr) {
-        mask_row = d.mask_rows[row];
     }
     bool bad = false;
     if (h1 < h0 || h1 > d.history_size) {
@@ -188,6 +196,24 @@ __global__ void __launch_bounds__(kThreads, 3) logits_process_kernel(const __gri
     }
     bool const penal = h1 > h0;
     bool const use_words = penal || b1 > b0;
+    // The thread's first 16-byte pieces of the history.
+    std::uint32_t const* const text = d.history + h0;
+    std::uint32_t const len = h1 - h0;
+    std::uint32_t const lead = (4u - static_cast<std::uint32_t>(reinterpret_cast<std::uintptr_t>(text) >> 2)) & 3u;
+    std::uint32_t const from = lead < len ? lead : len;
+    std::uint32_t const quads = (len - from) / 4u;
+    uint4 ahead[kQuads];
+    auto load_quads = [&](std::uint32_t q0) {
+#pragma unroll
+        for (std::uint32_t k = 0; k < kQuads; ++k) {
+            std::uint32_t const q = q0 + k * kThreads;
+            ahead[k] = make_uint4(0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu);  // no token
+            if (q < quads) {
+                ahead[k] = ldg_u4_now(text + from + q * 4u);
+            }
+        }
+    };
+    load_quads(tid);
     // The first bias of each thread, and the logit that it changes.
     std::uint32_t bias_token = 0, bias_next = 0xffffffffu;
     float bias_value = 0.f, bias_logit = 0.f;
@@ -220,58 +246,38 @@ __global__ void __launch_bounds__(kThreads, 3) logits_process_kernel(const __gri
     __syncthreads();
 
     // ---- the history and the biases
-    auto replace = [&](std::uint32_t at, float x) {
-        s_words[at] = __float_as_uint(x);
-        atomicOr(&s_touched[at / 32u], 1u << (at % 32u));
-    };
     if (penal) {
         auto count = [&](std::uint32_t at, std::uint32_t i) {
-            std::uint32_t const before = i < prompt ? atomicOr(&s_words[at], kPrompt) : atomicAdd(&s_words[at], 1u);
-            if (before == 0) {
-                std::uint32_t const n = atomicAdd(&s_listed, 1u);
-                if (n < kListed) {
-                    s_list[n] = static_cast<std::uint16_t>(at);
-                }
+            atomicOr(&s_touched[at / 32u], 1u << (at % 32u));
+            if (i >= prompt) {
+                atomicAdd(&s_words[at], 1u);
             }
         };
-        std::uint32_t const* const text = d.history + h0;
-        std::uint32_t const len = h1 - h0;
-        std::uint32_t const lead = (4u - static_cast<std::uint32_t>(reinterpret_cast<std::uintptr_t>(text) >> 2)) & 3u;
-        std::uint32_t const from = lead < len ? lead : len;
-        std::uint32_t const quads = (len - from) / 4u;
         for (std::uint32_t q0 = tid; q0 < quads; q0 += kThreads * kQuads) {
-            uint4 ahead[kQuads];
+            uint4 now[kQuads];
 #pragma unroll
             for (std::uint32_t k = 0; k < kQuads; ++k) {
-                std::uint32_t const q = q0 + k * kThreads;
-                if (q < quads) {
-                    ahead[k] = __ldg(reinterpret_cast<uint4 const*>(text + from) + q);
-                }
+                now[k] = ahead[k];
             }
+            load_quads(q0 + kThreads * kQuads);
 #pragma unroll
             for (std::uint32_t k = 0; k < kQuads; ++k) {
-                std::uint32_t const q = q0 + k * kThreads;
-                if (q >= quads) {
-                    break;
+                std::uint32_t const i = from + (q0 + k * kThreads) * 4u;
+                uint4 const t = now[k];
+                std::uint32_t const v[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+                for (std::uint32_t e = 0; e < 4u; ++e) {
+                    if (owned(v[e])) {
+                        count(place_of(v[e]), i + e);
+                    }
                 }
-                uint4 const t = ahead[k];
-                std::uint32_t mine = (owned(t.x) ? 1u : 0u) | (owned(t.y) ? 2u : 0u) | (owned(t.z) ? 4u : 0u)
-                    | (owned(t.w) ? 8u : 0u);
                 if (head != 0) {
-                    std::uint32_t const v[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
                     for (std::uint32_t e = 0; e < 4u; ++e) {
                         if (in_head(v[e])) {
-                            count(a.capacity + v[e], from + q * 4u + e);
+                            count(a.capacity + v[e], i + e);
                         }
                     }
-                }
-                // One token per thread and turn: about two turns a warp, not four.
-                while (mine != 0) {
-                    std::uint32_t const e = __ffs(mine) - 1u;
-                    mine &= mine - 1u;
-                    std::uint32_t const v = e < 2u ? (e == 0 ? t.x : t.y) : (e == 2u ? t.z : t.w);
-                    count(place_of(v), from + q * 4u + e);
                 }
             }
         }
@@ -287,37 +293,73 @@ __global__ void __launch_bounds__(kThreads, 3) logits_process_kernel(const __gri
         __syncthreads();
         auto logit_at = [&](std::uint32_t at) { return in[at < a.capacity ? token_of(at) : at - a.capacity]; };
         auto penalise = [&](std::uint32_t at, float x) {
-            std::uint32_t const n = s_words[at] & ~kPrompt;
+            std::uint32_t const n = s_words[at];
             x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
             if (n != 0) {
                 x = __fsub_rn(x, __fmul_rn(freq, static_cast<float>(n)));
                 x = __fsub_rn(x, pres);
             }
-            replace(at, x);
+            s_words[at] = __float_as_uint(x);
         };
-        std::uint32_t const listed = s_listed;
-        if (listed <= kListed) {
-            for (std::uint32_t i0 = tid; i0 < listed; i0 += kThreads * kQuads) {
-                std::uint32_t at[kQuads];
-                float x[kQuads];
+        // Marked tokens lie in clumps: they are spread over the threads by a list.
+        std::uint32_t const words = blocks * (kBlock / 32u);
+        for (std::uint32_t i0 = 0; i0 <= words; i0 += kThreads) {
+            std::uint32_t const i = i0 + tid;
+            std::uint32_t const w = i < words ? i : a.capacity / 32u;  // the head's word stands behind all blocks
+            std::uint32_t bits = i <= words ? s_touched[w] : 0u;
+            std::uint32_t const own = __popc(bits);
+            std::uint32_t upto = own;
 #pragma unroll
-                for (std::uint32_t k = 0; k < kQuads; ++k) {
-                    std::uint32_t const i = i0 + k * kThreads;
-                    at[k] = i < listed ? s_list[i] : 0u;
-                    x[k] = i < listed ? logit_at(at[k]) : 0.f;
+            for (std::uint32_t o = 1; o < 32u; o *= 2u) {
+                std::uint32_t const x = __shfl_up_sync(0xffffffffu, upto, o);
+                upto += tid % 32u >= o ? x : 0u;
+            }
+            std::uint32_t base = 0;
+            if (tid % 32u == 31u && upto != 0) {
+                base = atomicAdd(&s_listed, upto);
+            }
+            std::uint32_t n = __shfl_sync(0xffffffffu, base, 31) + upto - own;
+            auto list = [&](std::uint32_t at, std::uint32_t place) {
+                if (place < kListed) {
+                    s_list[place] = static_cast<std::uint16_t>(at);
+                } else {
+                    penalise(at, logit_at(at));
                 }
-#pragma unroll
-                for (std::uint32_t k = 0; k < kQuads; ++k) {
-                    if (i0 + k * kThreads < listed) {
-                        penalise(at[k], x[k]);
-                    }
+            };
+            // A word with many marks is taken by the whole warp, a lane a bit.
+            for (std::uint32_t full = __ballot_sync(0xffffffffu, own > 4u); full != 0; full &= full - 1u) {
+                std::uint32_t const from_lane = __ffs(full) - 1u;
+                std::uint32_t const word = __shfl_sync(0xffffffffu, bits, from_lane);
+                std::uint32_t const first = __shfl_sync(0xffffffffu, n, from_lane);
+                std::uint32_t const at = __shfl_sync(0xffffffffu, w, from_lane) * 32u + tid % 32u;
+                if ((word >> (tid % 32u) & 1u) != 0) {
+                    list(at, first + __popc(word & ((1u << (tid % 32u)) - 1u)));
                 }
             }
-        } else {
-            for (std::uint32_t i = tid; i < blocks * kBlock + head; i += kThreads) {
-                std::uint32_t const at = i < blocks * kBlock ? i : a.capacity + (i - blocks * kBlock);
-                if (s_words[at] != 0) {
-                    penalise(at, logit_at(at));
+            // Straight-line, as above: loops of divergent length cost three times as much.
+#pragma unroll
+            for (std::uint32_t e = 0; e < 4u; ++e) {
+                if (own <= 4u && bits != 0) {
+                    list(w * 32u + __ffs(bits) - 1u, n++);
+                    bits &= bits - 1u;
+                }
+            }
+        }
+        __syncthreads();
+        std::uint32_t const listed = s_listed < kListed ? s_listed : kListed;
+        for (std::uint32_t i0 = tid; i0 < listed; i0 += kThreads * kGather) {
+            std::uint32_t at[kGather];
+            float x[kGather];
+#pragma unroll
+            for (std::uint32_t k = 0; k < kGather; ++k) {
+                std::uint32_t const i = i0 + k * kThreads;
+                at[k] = i < listed ? s_list[i] : 0u;
+                x[k] = i < listed ? logit_at(at[k]) : 0.f;
+            }
+#pragma unroll
+            for (std::uint32_t k = 0; k < kGather; ++k) {
+                if (i0 + k * kThreads < listed) {
+                    penalise(at[k], x[k]);
                 }
             }
         }
@@ -335,7 +377,9 @@ __global__ void __launch_bounds__(kThreads, 3) logits_process_kernel(const __gri
         if ((low || owned(v)) && bias_next != v) {
             std::uint32_t const at = low ? a.capacity + v : place_of(v);
             bool const replaced = (s_touched[at / 32u] >> (at % 32u) & 1u) != 0;
-            replace(at, __fadd_rn(replaced ? __uint_as_float(s_words[at]) : bias_logit, bias_value));
+            s_words[at] = __float_as_uint(
+                __fadd_rn(replaced ? __uint_as_float(s_words[at]) : bias_logit, bias_value));
+            atomicOr(&s_touched[at / 32u], 1u << (at % 32u));
         }
     }
     if (b1 > b0) {
@@ -343,87 +387,90 @@ __global__ void __launch_bounds__(kThreads, 3) logits_process_kernel(const __gri
     }
 
     // ---- the logits
-    // A thread meets its tokens in ascending order, so a strict comparison
-    // keeps the lowest id of equal logits; NaN and -inf never pass it.
+    // The highest logit so far and where: a thread meets its steps of four tokens in
+    // ascending order, so a strict comparison keeps the lowest of equal ones; NaN
+    // and -inf never pass it.
     float top = -INFINITY;
     std::uint32_t top_id = 0;
-    auto offer = [&](float x, std::uint32_t v) {
-        if (x > top) {
-            top = x;
-            top_id = v;
-        }
-    };
     auto bits_of = [&](std::uint32_t const* bits, std::uint32_t at) { return bits[at / 32u] >> (at % 32u); };
-    auto one = [&](std::uint32_t at, std::uint32_t v, bool allowed) {
+    bool const masked = mask != nullptr || blocked;
+    std::uint64_t best = 0;  // of the tokens outside whole blocks
+    auto one = [&](std::uint32_t at, std::uint32_t v) {
+        bool const low = at >= a.capacity;
+        bool const allowed = !blocked
+            && (mask == nullptr || ((low ? mask[0] >> v : bits_of(s_mask, at)) & 1u) != 0);
         float x = use_words && (bits_of(s_touched, at) & 1u) != 0 ? __uint_as_float(s_words[at]) : in[v];
-        x = allowed && !blocked ? x : -INFINITY;
+        x = allowed ? x : -INFINITY;
+        std::uint64_t const c = candidate(x, v);
+        best = c > best ? c : best;
         if (out != nullptr) {
             out[v] = x;
         }
-        offer(x, v);
     };
     if (rank == 0 && tid < head) {
-        one(a.capacity + tid, tid, mask == nullptr || (mask[0] >> tid & 1u) != 0);
+        one(a.capacity + tid, tid);
     }
-    std::uint32_t const steps = blocks * (kBlock / 4u);
-    for (std::uint32_t i0 = tid; i0 < steps; i0 += kThreads * kVecs) {
-        float4 x[kVecs];
+    // A warp takes a block of 256 tokens: two steps of four for every thread. The
+    // places of consecutive blocks of a warp lie kWarps blocks apart, their
+    // tokens that times the cluster's size.
+    std::uint32_t const lane4 = (tid % 32u) * 4u;
+    std::uint32_t const whole_blocks = blocks != 0 && token_of((blocks - 1u) * kBlock) + kBlock > vocab ? blocks - 1u : blocks;
+    {
+        std::uint32_t at = tid / 32u * kBlock + lane4;
+        std::uint32_t v = head + ((tid / 32u << lc) + rank) * kBlock + lane4;
+        std::uint32_t const stride = (kWarps * kBlock) << lc;
+        bool const vector_out = out != nullptr && same_phase;
+        for (std::uint32_t block = tid / 32u; block < whole_blocks; block += kWarps, at += kWarps * kBlock, v += stride) {
+            float4 x[2] = {*reinterpret_cast<float4 const*>(in + v), *reinterpret_cast<float4 const*>(in + v + 128u)};
+            if (use_words) {
 #pragma unroll
-        for (std::uint32_t k = 0; k < kVecs; ++k) {
-            std::uint32_t const i = i0 + k * kThreads;
-            std::uint32_t const v = token_of(i * 4u);
-            if (i < steps && v + 4u <= vocab) {
-                x[k] = *reinterpret_cast<float4 const*>(in + v);
+                for (std::uint32_t k = 0; k < 2u; ++k) {
+                    std::uint32_t const marked = bits_of(s_touched, at + k * 128u) & 15u;
+                    if (marked != 0) {
+                        uint4 const w = *reinterpret_cast<uint4 const*>(&s_words[at + k * 128u]);
+                        x[k].x = (marked & 1u) != 0 ? __uint_as_float(w.x) : x[k].x;
+                        x[k].y = (marked & 2u) != 0 ? __uint_as_float(w.y) : x[k].y;
+                        x[k].z = (marked & 4u) != 0 ? __uint_as_float(w.z) : x[k].z;
+                        x[k].w = (marked & 8u) != 0 ? __uint_as_float(w.w) : x[k].w;
+                    }
+                }
+            }
+            if (masked) {
+#pragma unroll
+                for (std::uint32_t k = 0; k < 2u; ++k) {
+                    std::uint32_t const allow = blocked ? 0u : bits_of(s_mask, at + k * 128u);
+                    x[k].x = (allow & 1u) != 0 ? x[k].x : -INFINITY;
+                    x[k].y = (allow & 2u) != 0 ? x[k].y : -INFINITY;
+                    x[k].z = (allow & 4u) != 0 ? x[k].z : -INFINITY;
+                    x[k].w = (allow & 8u) != 0 ? x[k].w : -INFINITY;
+                }
+            }
+#pragma unroll
+            for (std::uint32_t k = 0; k < 2u; ++k) {
+                float const high = fmaxf(fmaxf(fmaxf(x[k].x, x[k].y), x[k].z), x[k].w);  // passes NaN over
+                if (high > top) {
+                    top = high;
+                    top_id = v + k * 128u + (x[k].x == high ? 0u : x[k].y == high ? 1u : x[k].z == high ? 2u : 3u);
+                }
+            }
+            if (vector_out) {
+                *reinterpret_cast<float4*>(out + v) = x[0];
+                *reinterpret_cast<float4*>(out + v + 128u) = x[1];
+            } else if (out != nullptr) {
+#pragma unroll
+                for (std::uint32_t k = 0; k < 2u; ++k) {
+                    out[v + k * 128u] = x[k].x;
+                    out[v + k * 128u + 1u] = x[k].y;
+                    out[v + k * 128u + 2u] = x[k].z;
+                    out[v + k * 128u + 3u] = x[k].w;
+                }
             }
         }
-#pragma unroll
-        for (std::uint32_t k = 0; k < kVecs; ++k) {
-            std::uint32_t const i = i0 + k * kThreads;
-            std::uint32_t const at = i * 4u;
-            std::uint32_t const v = token_of(at);
-            if (i >= steps || v >= vocab) {
-                continue;
-            }
-            std::uint32_t allow = blocked ? 0u : 15u;
-            if (mask != nullptr) {
-                allow = bits_of(s_mask, at);
-            }
-            if (v + 4u > vocab) {  // the last, partial step
-                for (std::uint32_t e = 0; v + e < vocab; ++e) {
-                    one(at + e, v + e, (allow >> e & 1u) != 0);
-                }
-                continue;
-            }
-            if (use_words) {
-                std::uint32_t const replaced = bits_of(s_touched, at) & 15u;
-                if (replaced != 0) {
-                    uint4 const w = *reinterpret_cast<uint4 const*>(&s_words[at]);
-                    x[k].x = (replaced & 1u) != 0 ? __uint_as_float(w.x) : x[k].x;
-                    x[k].y = (replaced & 2u) != 0 ? __uint_as_float(w.y) : x[k].y;
-                    x[k].z = (replaced & 4u) != 0 ? __uint_as_float(w.z) : x[k].z;
-                    x[k].w = (replaced & 8u) != 0 ? __uint_as_float(w.w) : x[k].w;
-                }
-            }
-            x[k].x = (allow & 1u) != 0 ? x[k].x : -INFINITY;
-            x[k].y = (allow & 2u) != 0 ? x[k].y : -INFINITY;
-            x[k].z = (allow & 4u) != 0 ? x[k].z : -INFINITY;
-            x[k].w = (allow & 8u) != 0 ? x[k].w : -INFINITY;
-            if (d.tokens != nullptr) {
-                offer(x[k].x, v);
-                offer(x[k].y, v + 1u);
-                offer(x[k].z, v + 2u);
-                offer(x[k].w, v + 3u);
-            }
-            if (out != nullptr) {
-                if (same_phase) {
-                    *reinterpret_cast<float4*>(out + v) = x[k];
-                } else {
-                    out[v] = x[k].x;
-                    out[v + 1u] = x[k].y;
-                    out[v + 2u] = x[k].z;
-                    out[v + 3u] = x[k].w;
-                }
-            }
+    }
+    if (whole_blocks < blocks) {  // the vocabulary's last, partial block
+        std::uint32_t const at0 = whole_blocks * kBlock;
+        for (std::uint32_t e = tid; token_of(at0) + e < vocab; e += kThreads) {
+            one(at0 + e, token_of(at0) + e);
         }
     }
 
@@ -431,7 +478,8 @@ __global__ void __launch_bounds__(kThreads, 3) logits_process_kernel(const __gri
     if (d.tokens == nullptr) {
         return;
     }
-    std::uint64_t best = candidate(top, top_id);
+    std::uint64_t const whole = candidate(top, top_id);
+    best = whole > best ? whole : best;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         std::uint64_t const other = __shfl_xor_sync(0xffffffffu, best, o);
@@ -442,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, 3) logits_process_kernel(const __gri
     }
     __syncthreads();
     if (tid == 0) {
-        for (std::uint32_t w = 1; w < kThreads / 32u; ++w) {
+        for (std::uint32_t w = 1; w < kWarps; ++w) {
             best = s_best[w] > best ? s_best[w] : best;
         }
     }

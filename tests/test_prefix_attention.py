@@ -314,8 +314,9 @@ class Setup:
         top = float(torch.einsum("hgd,thd->hgt", q.abs(), k.abs()).max()) * self.scale
         # A score is a sum of 64 products in FP32 (2^-23 a step at most): a weight is off by 2^-17 top
         # relative, and by 2^-21 for the exponential and its argument; a quotient of two such sums by
-        # twice that. Sums over T tokens add 2^-23 a token. All of it scales with the largest value.
-        size = float(v.abs().max()) * (2 * (top * 2.0 ** -17 + 2.0 ** -21) + (k.shape[0] + 64) * 2.0 ** -23)
+        # twice that. A weight of a shared token is rounded to FP16, off by 2^-11 at most. Sums over T
+        # tokens add 2^-23 a token. All of it scales with the largest value.
+        size = float(v.abs().max()) * (2 * (top * 2.0 ** -17 + 2.0 ** -21) + 2.0 ** -11 + (k.shape[0] + 64) * 2.0 ** -23)
         return out, size
 
     def check(self, layer=1):
