@@ -290,10 +290,10 @@ __device__ __forceinline__ std::uint64_t add_f32x2(std::uint64_t a, std::uint64_
     return r;
 }
 
-__device__ __forceinline__ float max_nan(float a, float b)  // NaN if either is
+__device__ __forceinline__ float max_nan(float a, float b, float c)  // NaN if one of them is
 {
     float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
 
@@ -331,6 +331,14 @@ __device__ __forceinline__ std::uint32_t pack_half2(float lo, float hi)
 
 // The leading 11 bits of p: what FP16 holds of it exactly (above its subnormals).
 __device__ __forceinline__ float leading(float p) { return __uint_as_float(__float_as_uint(p) & 0xffffe000u); }
+
+// Partials are rows of 16 chunks of 16 bytes; a row's chunks are permuted by its
+// number, so that a thread per row can write them to shared memory without bank
+// conflicts. Place of chunk c:
+__device__ __forceinline__ std::uint32_t part_chunk(std::uint64_t row, std::uint32_t c)
+{
+    return c ^ (static_cast<std::uint32_t>(row) & 15u);
+}
 
 // ---- shared items -------------------------------------------------------------
 
@@ -613,9 +621,9 @@ __device__ __forceinline__ void soften(Args const& a, kk_prefix_item const& item
             float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
             for (std::uint32_t i = 0; i < kTile; i += 2u) {
-                top[i / 2u % 4u] = max_nan(max_nan(top[i / 2u % 4u], x[i]), x[i + 1u]);
+                top[i / 2u % 4u] = max_nan(top[i / 2u % 4u], x[i], x[i + 1u]);
             }
-            float const mt = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3])) * a.scale_log2;
+            float const mt = max_nan(max_nan(top[0], top[1], top[2]), top[3], top[3]) * a.scale_log2;
             bool const grow = mt > m + kRescale || m == -INFINITY;
             if (__any_sync(0xffffffffu, grow)) {
                 float const now = grow ? mt : m;
@@ -685,7 +693,7 @@ __device__ __forceinline__ void soften(Args const& a, kk_prefix_item const& item
     // One row tile: the second group's O joins the first's through the ring,
     // which nothing uses any more.
     constexpr std::uint32_t kStride = kHeadDim + 3;  // odd: rows fall into different banks
-    static_assert(kTile * kStride * 4 <= kStages * kStageBytes, "room for one O tile");
+    static_assert(kTile * kStride * 4 <= 2 * kStageBytes, "room below the tiles that leave");
     float* const other = reinterpret_cast<float*>(ring) + r * kStride;
     if (!pair && t == 1u && ok) {
         bool const holds = any && turns > 1u;
@@ -704,11 +712,11 @@ __device__ __forceinline__ void soften(Args const& a, kk_prefix_item const& item
         other[kHeadDim + 1] = l;
     }
     asm volatile("bar.sync 1, 256;" ::: "memory");  // the 8 softmax warps, all of which come here
-    if ((!pair && t == 1u) || !ok || !any) {
+    if (!pair && t == 1u) {
         return;
     }
     float f0 = 1.f, f1 = 0.f;
-    if (!pair) {
+    if (!pair && ok) {
         float const m1 = other[kHeadDim];
         float const top = fmaxf(m, m1);
         float const use = top == -INFINITY ? 0.f : top;
@@ -717,27 +725,41 @@ __device__ __forceinline__ void soften(Args const& a, kk_prefix_item const& item
         m = top;
         l = l * f0 + other[kHeadDim + 1] * f1;
     }
-    std::uint64_t const row = std::uint64_t(item.part_row) + (t & pair) * kTile + r;
-    float4* const dst = reinterpret_cast<float4*>(a.part_o + row * kHeadDim);
+    // The rows leave through shared memory in one bulk copy (stores of a row per
+    // thread took 3.4 us in place of 0.9 for two row tiles).
+    std::uint64_t const first_row = std::uint64_t(item.part_row) + (t & pair) * kTile;
+    float4* const tile = reinterpret_cast<float4*>(ring + (2u + t) * kStageBytes);
+    if (ok && any) {
 #pragma unroll
-    for (std::uint32_t c = 0; c < 4u; ++c) {
-        float o[16];
-        tmem_ld16(o_col + c * 16u, o);  // the whole warp, also for rows that do not exist
-        if (!pair) {
+        for (std::uint32_t c = 0; c < 4u; ++c) {
+            float o[16];
+            tmem_ld16(o_col + c * 16u, o);  // the whole warp, also for rows that do not exist
+            if (!pair) {
 #pragma unroll
-            for (std::uint32_t i = 0; i < 16u; ++i) {
-                o[i] = o[i] * f0 + other[c * 16u + i] * f1;
+                for (std::uint32_t i = 0; i < 16u; ++i) {
+                    o[i] = o[i] * f0 + other[c * 16u + i] * f1;
+                }
+            }
+#pragma unroll
+            for (std::uint32_t i = 0; i < 4u; ++i) {
+                tile[r * 16u + part_chunk(first_row + r, c * 4u + i)] =
+                    make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
             }
         }
         if (mine) {
-#pragma unroll
-            for (std::uint32_t i = 0; i < 4u; ++i) {
-                dst[c * 4u + i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-            }
+            a.part_ml[first_row + r] = make_float2(m, l);
         }
     }
-    if (mine) {
-        a.part_ml[row] = make_float2(m, l);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    asm volatile("bar.sync %0, 128;" ::"r"(2u + t) : "memory");  // the group's 4 warps, all of which come here
+    if (r == 0 && !*abort) {
+        std::uint32_t const left = rows - tile_row;
+        std::uint32_t const bytes = (left < kTile ? left : kTile) * kHeadDim * 4u;
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;"
+                     ::"l"(a.part_o + first_row * kHeadDim), "r"(smem_u32(tile)), "r"(bytes)
+                     : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     }
 }
 
@@ -985,11 +1007,11 @@ __device__ __forceinline__ void own_task(Args const& a, kk_prefix_item const& it
             l += __shfl_xor_sync(0xffffffffu, l, 16);
             std::uint32_t const qh = nt * 8u + 2u * c4 + h;
             if (qh < G) {
-                float* dst = a.part_o + (row0 + qh) * kHeadDim;
+                float* dst = a.part_o + (row0 + qh) * kHeadDim + g % 4u;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    dst[16 * j + g] = o[nt][j][h];
-                    dst[16 * j + 8 + g] = o[nt][j][2 + h];
+                for (std::uint32_t j = 0; j < 4u; ++j) {
+                    dst[part_chunk(row0 + qh, 4u * j + g / 4u) * 4u] = o[nt][j][h];
+                    dst[part_chunk(row0 + qh, 4u * j + 2u + g / 4u) * 4u] = o[nt][j][2 + h];
                 }
                 if (g == 0) {
                     a.part_ml[row0 + qh] = make_float2(mrow[nt][h], l);
@@ -1103,20 +1125,21 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_attention_kernel(const __g
 constexpr std::uint32_t kJoinThreads = 256;
 constexpr std::uint32_t kJoinBatch = 8;  // partials requested at once
 
-// 16 threads per query row, 4 dims each: out = sum_i 2^(m_i - m) O_i / sum_i
-// 2^(m_i - m) l_i over the row's partials, in their order.
+// A warp per query row: out = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i over the
+// row's partials. 16 lanes hold 4 dims each; the two halves of the warp take
+// alternate partials, kJoinBatch of them at a time, and join in a fixed order.
 __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(const __grid_constant__ Args a)
 {
     std::uint32_t const t = blockIdx.x * kJoinThreads + threadIdx.x;
     std::uint32_t const q_heads = a.plan.q_heads;
-    std::uint32_t const lane = t / 16u / q_heads;
+    std::uint32_t const lane = t / 32u / q_heads;
     if (lane >= a.plan.num_lanes) {
         return;
     }
     // The plan is older than the launch that writes the partials: it is read
     // before that one has ended.
-    std::uint32_t const qh = t / 16u % q_heads;
-    std::uint32_t const d0 = t % 16u * 4u;
+    std::uint32_t const qh = t / 32u % q_heads;
+    std::uint32_t const chunk = t % 16u;
     kk_attn_lane const ln = a.lanes[lane];
     std::uint64_t base = 0, step = 0;
     std::uint32_t shared = 0;
@@ -1138,39 +1161,54 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(const __grid_
     pdl_wait();
     float m = -INFINITY, l = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (std::uint32_t i0 = 0; i0 < count; i0 += kJoinBatch) {
+    auto add = [&](float m1, float l1, float4 const& o) {
+        float const top = fmaxf(m, m1);
+        float const use = top == -INFINITY ? 0.f : top;
+        float const f = exp2_approx(m - use);
+        float const f1 = exp2_approx(m1 - use);
+        m = top;
+        l = l * f + l1 * f1;
+        acc.x = acc.x * f + o.x * f1;
+        acc.y = acc.y * f + o.y * f1;
+        acc.z = acc.z * f + o.z * f1;
+        acc.w = acc.w * f + o.w * f1;
+    };
+    for (std::uint32_t i0 = t % 32u / 16u; i0 < count; i0 += 2u * kJoinBatch) {
         float2 ml[kJoinBatch];
         float4 o[kJoinBatch];
 #pragma unroll
         for (std::uint32_t k = 0; k < kJoinBatch; ++k) {
-            std::uint32_t const i = i0 + k;
+            std::uint32_t const i = i0 + 2u * k;
             ml[k] = make_float2(-INFINITY, 0.f);
             o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
             if (i < count) {
                 std::uint64_t const row = i < shared ? base + i * step : own + std::uint64_t(i - shared) * q_heads;
                 ml[k] = __ldcg(a.part_ml + row);
-                o[k] = __ldcg(reinterpret_cast<float4 const*>(a.part_o + row * kHeadDim + d0));
+                o[k] = __ldcg(reinterpret_cast<float4 const*>(a.part_o + row * kHeadDim) + part_chunk(row, chunk));
             }
         }
 #pragma unroll
         for (std::uint32_t k = 0; k < kJoinBatch; ++k) {
-            float const m_new = fmaxf(m, ml[k].x);
-            float const use = m_new == -INFINITY ? 0.f : m_new;
-            float const f = exp2_approx(m - use);
-            float const fk = exp2_approx(ml[k].x - use);
-            m = m_new;
-            l = l * f + ml[k].y * fk;
-            acc.x = acc.x * f + o[k].x * fk;
-            acc.y = acc.y * f + o[k].y * fk;
-            acc.z = acc.z * f + o[k].z * fk;
-            acc.w = acc.w * f + o[k].w * fk;
+            add(ml[k].x, ml[k].y, o[k]);
         }
     }
+    // The upper half's part joins the lower's.
+    float const m1 = __shfl_down_sync(0xffffffffu, m, 16);
+    float const l1 = __shfl_down_sync(0xffffffffu, l, 16);
+    float4 o1;
+    o1.x = __shfl_down_sync(0xffffffffu, acc.x, 16);
+    o1.y = __shfl_down_sync(0xffffffffu, acc.y, 16);
+    o1.z = __shfl_down_sync(0xffffffffu, acc.z, 16);
+    o1.w = __shfl_down_sync(0xffffffffu, acc.w, 16);
+    if (t % 32u >= 16u) {
+        return;
+    }
+    add(m1, l1, o1);
     float const inv = l == 0.f ? 0.f : 1.f / l;  // no tokens at all: zeros
     uint2 out;
     out.x = pack_half2(acc.x * inv, acc.y * inv);
     out.y = pack_half2(acc.z * inv, acc.w * inv);
-    *reinterpret_cast<uint2*>(a.output + ln.query_row * a.output_stride + qh * kHeadDim + d0) = out;
+    *reinterpret_cast<uint2*>(a.output + ln.query_row * a.output_stride + qh * kHeadDim + chunk * 4u) = out;
 }
 
 // Kernel attributes are set once per device.
@@ -1203,11 +1241,15 @@ cudaError_t allowSharedMemory()
 
 // ---- planning -------------------------------------------------------------------
 
-// Measured costs of a thread block's work, in nanoseconds, that decide how
-// many splits the prefixes get against the lanes' own pages.
-constexpr double kTilePairNs = 1200.;   // a 128-token tile for two row tiles
-constexpr double kTileSingleNs = 620.;  // for one
-constexpr double kOwnTokenNs = 5.7;     // a token of one KV head: 256 bytes at an SM's share of HBM
+// Measured times of a thread block, in nanoseconds, from which the plan deals
+// the SMs out between the prefixes and the lanes' own pages.
+constexpr double kSharedNs = 5500.;     // a shared item without its tiles
+constexpr double kTilePairNs = 1450.;   // a 128-token tile for two row tiles
+constexpr double kTileSingleNs = 750.;  // for one
+constexpr double kOwnNs = 1000.;        // a block of lanes' own items without them
+constexpr double kTaskNs = 2200.;       // an own item without its tokens
+constexpr double kTaskTokenNs = 28.;     // a token of an own item, by its warp
+constexpr double kOwnTokenNs = 6.;      // the same by the block: 256 bytes at an SM's share of HBM
 constexpr std::uint32_t kOwnMinTokens = 64;
 
 std::uint32_t groupsOf(kk_page_desc const& d) { return d.valid_tokens > 64u ? 0u : (d.valid_tokens + 7u) / 8u; }
@@ -1304,6 +1346,8 @@ int kk_prefix_attention_plan(const kk_page_desc* descs, uint32_t num_descs, kk_a
     auto outside = [&](std::uint32_t offset, std::uint32_t count) {
         return offset > num_descs || count > num_descs - offset;
     };
+    // Tokens of a lane's own pages, in whole groups, stand in item_offset, and tiles
+    // of a prefix in part_row, until the plan is made.
     std::uint64_t own_tokens = 0;
     for (std::uint32_t b = 0; b < num_lanes; ++b) {
         kk_attn_lane& ln = lanes[b];
@@ -1311,16 +1355,18 @@ int kk_prefix_attention_plan(const kk_page_desc* descs, uint32_t num_descs, kk_a
             return KK_EINVAL;
         }
         ln.item_offset = ln.item_count = ln.reserved = 0;
+        std::uint64_t tokens = 0;
         for (std::uint32_t e = ln.desc_offset; e < ln.desc_offset + ln.desc_count; ++e) {
-            own_tokens += 8u * groupsOf(descs[e]);
+            tokens += 8u * groupsOf(descs[e]);
         }
+        if (tokens > 0xffffffffull) {
+            return KK_EINVAL;
+        }
+        ln.item_offset = static_cast<std::uint32_t>(tokens);
+        own_tokens += tokens;
     }
-    // A prefix's tiles and what one KV head's rows cost on it.
-    auto tilesOf = [&](kk_prefix_group const& g) {
-        return walkTiles(descs, g.desc_offset, g.desc_offset + g.desc_count, [](std::uint32_t, std::uint32_t) {});
-    };
-    auto unitNs = [](kk_prefix_group const& g) { return g.row_tiles > 1u ? kTilePairNs : kTileSingleNs; };
-    double total = static_cast<double>(own_tokens) * kv_heads * kOwnTokenNs;
+    auto tileNs = [](kk_prefix_group const& g) { return g.row_tiles > 1u ? kTilePairNs : kTileSingleNs; };
+    double longest = 0.;
     for (std::uint32_t i = 0; i < num_groups; ++i) {
         kk_prefix_group& g = groups[i];
         if (outside(g.desc_offset, g.desc_count) || g.lane_begin > num_lanes
@@ -1338,10 +1384,53 @@ int kk_prefix_attention_plan(const kk_page_desc* descs, uint32_t num_descs, kk_a
             }
             lanes[b].reserved = i + 1u;
         }
-        total += static_cast<double>(tilesOf(g)) * ((g.row_tiles + 1u) / 2u) * kv_heads * unitNs(g);
+        g.part_row = walkTiles(descs, g.desc_offset, g.desc_offset + g.desc_count, [](std::uint32_t, std::uint32_t) {});
+        longest = std::fmax(longest, kSharedNs + g.part_row * tileNs(g));
     }
-    // One thread block per SM, all of about the same cost.
-    double const share = total / num_sms;
+    // The shortest time in which num_sms blocks, one to an SM, can do the work.
+    auto partsIn = [&](kk_prefix_group const& g, double ns) {
+        double const most = std::fmax(1., std::floor((ns - kSharedNs) / tileNs(g)));
+        return static_cast<std::uint32_t>(std::ceil(g.part_row / most));
+    };
+    auto taskTokensIn = [&](double ns) {
+        return std::fmax(kOwnMinTokens, std::floor((ns - kOwnNs - kTaskNs) / kTaskTokenNs));
+    };
+    auto tasksOf = [&](double per_task) {
+        double tasks = 0.;
+        for (std::uint32_t b = 0; b < num_lanes; ++b) {
+            tasks += std::ceil(lanes[b].item_offset / per_task) * kv_heads;
+        }
+        return tasks;
+    };
+    auto roundsIn = [&](double ns, double tasks) {  // items that a warp does one after the other
+        double const tokens = static_cast<double>(own_tokens) * kv_heads;
+        return std::fmax(1., std::floor((ns - kOwnNs) / (kTaskNs + kTaskTokenNs * tokens / tasks)));
+    };
+    auto ownBlocksIn = [&](double ns) {
+        if (own_tokens == 0) {
+            return 0.;
+        }
+        double const tasks = tasksOf(taskTokensIn(ns));
+        double const tokens = static_cast<double>(own_tokens) * kv_heads;
+        double const rounds = roundsIn(ns, tasks);
+        return std::fmax(std::ceil(tasks / (rounds * kSoftWarps)),
+            std::ceil(tokens * kOwnTokenNs / std::fmax(1., ns - kOwnNs - kTaskNs)));
+    };
+    auto sharedBlocksIn = [&](double ns) {
+        double blocks = 0.;
+        for (std::uint32_t i = 0; i < num_groups; ++i) {
+            blocks += static_cast<double>(partsIn(groups[i], ns)) * kv_heads * ((groups[i].row_tiles + 1u) / 2u);
+        }
+        return blocks;
+    };
+    double lo = 0., hi = std::fmax(longest, kOwnNs + kTaskNs + kTaskTokenNs * 0x1p32);
+    for (int i = 0; i < 48; ++i) {
+        double const mid = 0.5 * (lo + hi);
+        bool const done = mid >= kSharedNs && mid >= kOwnNs + kTaskNs
+            && sharedBlocksIn(mid) + ownBlocksIn(mid) <= num_sms;
+        (done ? hi : lo) = mid;
+    }
+    double const time = hi;
     std::uint32_t count = 0;
     std::uint64_t part_rows = 0;
     auto put = [&](kk_prefix_item const& item) {
@@ -1352,13 +1441,12 @@ int kk_prefix_attention_plan(const kk_page_desc* descs, uint32_t num_descs, kk_a
     };
     for (std::uint32_t i = 0; i < num_groups; ++i) {
         kk_prefix_group& g = groups[i];
-        std::uint32_t const tiles = tilesOf(g);
+        std::uint32_t const tiles = g.part_row;
+        std::uint32_t const parts = tiles != 0 ? partsIn(g, time) : 0u;
         g.part_row = g.part_count = 0;
         if (tiles == 0 || g.row_tiles == 0) {
             continue;
         }
-        double const want = std::floor(tiles * unitNs(g) / share);
-        std::uint32_t const parts = want < 1. ? 1u : want > tiles ? tiles : static_cast<std::uint32_t>(want);
         g.part_count = parts;
         std::uint64_t const rows = std::uint64_t(kv_heads) * parts * g.row_tiles * kTile;
         if (part_rows + rows > 0xffffffffull) {
@@ -1388,21 +1476,25 @@ int kk_prefix_attention_plan(const kk_page_desc* descs, uint32_t num_descs, kk_a
     }
     plan->num_shared = count;
     if (own_tokens != 0) {
-        double const own_ns = static_cast<double>(own_tokens) * kv_heads * kOwnTokenNs;
-        std::uint32_t ctas = static_cast<std::uint32_t>(std::ceil(own_ns / share));
-        if (count < num_sms && ctas < num_sms - count) {
-            ctas = num_sms - count;
+        // What the prefixes leave of the SMs, and no less than the plan set aside.
+        std::uint32_t blocks = static_cast<std::uint32_t>(std::fmin(ownBlocksIn(time), 1e6));
+        blocks = blocks < 1u ? 1u : blocks;
+        if (count < num_sms && blocks < num_sms - count) {
+            blocks = num_sms - count;
         }
-        std::uint64_t const warps = std::uint64_t(ctas) * kSoftWarps;
-        std::uint64_t per_task = (own_tokens * kv_heads + warps - 1u) / warps;
-        per_task = per_task < kOwnMinTokens ? kOwnMinTokens : per_task;
+        // The shortest items that those blocks take in as many rounds.
+        double const longest_task = taskTokensIn(time);
+        double const room = std::floor(roundsIn(time, tasksOf(longest_task))) * blocks * kSoftWarps;
+        double tokens = kOwnMinTokens;
+        while (tokens < longest_task && tasksOf(tokens) > room) {
+            tokens *= 1.125;
+        }
+        std::uint64_t const per_task = static_cast<std::uint64_t>(std::fmin(std::ceil(tokens), longest_task));
         for (std::uint32_t b = 0; b < num_lanes; ++b) {
             kk_attn_lane& ln = lanes[b];
             std::uint32_t const end = ln.desc_offset + ln.desc_count;
-            std::uint64_t len = 0;
-            for (std::uint32_t e = ln.desc_offset; e < end; ++e) {
-                len += 8u * groupsOf(descs[e]);
-            }
+            std::uint64_t const len = ln.item_offset;
+            ln.item_offset = 0;
             if (len == 0) {
                 continue;
             }
@@ -1429,7 +1521,7 @@ int kk_prefix_attention_plan(const kk_page_desc* descs, uint32_t num_descs, kk_a
             }
         }
         std::uint32_t const tasks = count - plan->num_shared;
-        std::uint32_t const per_cta = (tasks + ctas - 1u) / ctas;
+        std::uint32_t const per_cta = (tasks + blocks - 1u) / blocks;
         plan->tasks_per_cta = per_cta < kSoftWarps ? kSoftWarps : per_cta;
     }
     plan->num_items = count;
@@ -1467,7 +1559,7 @@ int kk_prefix_attention(const kk_prefix_attn_desc* d, void* stream)
                 || d->workspace_bytes < kk_prefix_attention_workspace_bytes(&d->plan)))) {
         return KK_EINVAL;
     }
-    std::uint64_t const threads = std::uint64_t(d->plan.num_lanes) * d->q_heads * 16u;
+    std::uint64_t const threads = std::uint64_t(d->plan.num_lanes) * d->q_heads * 32u;
     if (threads > 0xffffffffull) {
         return KK_EINVAL;
     }
