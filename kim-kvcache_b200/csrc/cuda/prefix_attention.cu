@@ -11,7 +11,7 @@
 // row's partials and rounds once to FP16.
 //
 // Shared item (one block per SM), up to two tiles of 128 query rows:
-//  * warp 8 walks the item's descriptors and fills a 4-stage ring with 128-token
+//  * warp 8 walks the item's descriptors and fills a 6-stage ring with 128-token
 //    tiles of one KV head, K then V, [token][64 dims] with the 128-byte
 //    swizzle (TMA; an 8-token group is one swizzle atom, so pages of any size
 //    meet in a tile; each lane issues the copies of one page). A tile that is
@@ -56,7 +56,8 @@ namespace {
 
 constexpr std::uint32_t kHeadDim = 64;
 constexpr std::uint32_t kRowBytes = kHeadDim * 2;
-constexpr std::uint32_t kSoftWarps = 8;               // also of a block that serves lanes' own pages
+constexpr std::uint32_t kSoftWarps = 8;
+constexpr std::uint32_t kOwnWarps = 8;                // of a block that serves lanes' own pages
 constexpr std::uint32_t kProducerWarp = 8;
 constexpr std::uint32_t kIssuerWarp = 9;
 constexpr std::uint32_t kThreads = 384;               // three warpgroups; warps 10 and 11 only fill the third
@@ -67,7 +68,7 @@ constexpr std::uint32_t kLaunchRegs = 168;
 constexpr std::uint32_t kSoftRegs = 216;
 constexpr std::uint32_t kFewRegs = 72;
 static_assert(2 * kSoftRegs + kFewRegs <= 3 * kLaunchRegs, "a share beyond the launch's registers never comes");
-constexpr std::uint32_t kStages = 4;
+constexpr std::uint32_t kStages = 6;
 constexpr std::uint32_t kTile = 128;                  // tokens per tile, and query rows per row tile
 constexpr std::uint32_t kSlots = kTile / 8;           // 8-token groups per tile
 constexpr std::uint32_t kTileBytes = kTile * kRowBytes;  // K, V or Q
@@ -84,8 +85,8 @@ constexpr std::uint32_t kColO = 384;    // two O tiles of 64
 // A lane's own pages.
 constexpr std::uint32_t kSlice = 16;                       // tokens per step
 constexpr std::uint32_t kSliceBytes = 2 * kSlice * kRowBytes;
-constexpr std::uint32_t kSliceRing = kStages * kStageBytes / kSoftWarps / kSliceBytes;  // 4
-static_assert(kSliceRing == 4, "the validity queue below holds four slices");
+constexpr std::uint32_t kSliceRing = kStages * kStageBytes / kOwnWarps / kSliceBytes;  // 6
+static_assert(kSliceRing <= 9, "the validity queue below holds eight slices");
 
 // Of kPolyOf pairs of weights, kPoly are computed without the exponential unit.
 // Measured on 64 lanes over two prefixes of 32,749 tokens: 59.6 us with none,
@@ -877,7 +878,7 @@ __device__ __forceinline__ void own_task(Args const& a, kk_prefix_item const& it
         return 0u;
     };
     std::uint32_t const ring = smem_u32(warp_ring);
-    std::uint32_t queue = 0;  // valid tokens of the slices in flight: 8 bits each, newest highest
+    std::uint64_t queue = 0;  // valid tokens of the slices in flight: 8 bits each, newest highest
     std::uint32_t head_slice = 0;  // slices requested
     auto request = [&]() {  // one slice (or nothing) into the ring, always one commit group
         __half const* at0 = nullptr;
@@ -899,7 +900,7 @@ __device__ __forceinline__ void own_task(Args const& a, kk_prefix_item const& it
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        queue = (queue >> 8) | ((v0 | (v1 << 4)) << 24);
+        queue = (queue >> 8) | (std::uint64_t(v0 | (v1 << 4)) << 56);
         ++head_slice;
     };
     float mrow[NT][2], lrow[NT][2], o[NT][4][4];
@@ -912,17 +913,18 @@ __device__ __forceinline__ void own_task(Args const& a, kk_prefix_item const& it
             o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
         }
     }
-    request();
-    request();
-    request();
+#pragma unroll 1
+    for (std::uint32_t i = 0; i + 1u < kSliceRing; ++i) {
+        request();
+    }
     for (std::uint32_t slice = 0;; ++slice) {
-        // The slice in turn is the third newest; it is the oldest with tokens left.
-        std::uint32_t const pairv = (queue >> 8) & 0xffu;
+        // The slice in turn is the oldest of the kSliceRing - 1 requested last.
+        std::uint32_t const pairv = static_cast<std::uint32_t>(queue >> (64u - 8u * (kSliceRing - 1u))) & 0xffu;
         if (pairv == 0) {
             break;
         }
         request();
-        asm volatile("cp.async.wait_group 3;" ::: "memory");
+        asm volatile("cp.async.wait_group %0;" ::"n"(kSliceRing - 1u) : "memory");
         __syncwarp();
         std::uint32_t const v0 = pairv & 15u, v1 = pairv >> 4;
         std::uint32_t const kbase = ring + (slice % kSliceRing) * kSliceBytes;
@@ -950,27 +952,41 @@ __device__ __forceinline__ void own_task(Args const& a, kk_prefix_item const& it
         std::uint32_t pb[NT][2], pl[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
+            float x[4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                x[h] = tg ? st[nt][h] * a.scale_log2 : -INFINITY;
+                x[2 + h] = tg8 ? st[nt][2 + h] * a.scale_log2 : -INFINITY;
+            }
+            // As in the shared items, the reference follows the maximum only when
+            // that has grown by 2^8: a vote in place of two reductions a slice.
+            float const top0 = fmaxf(x[0], x[2]), top1 = fmaxf(x[1], x[3]);
+            if (__any_sync(0xffffffffu, top0 > mrow[nt][0] + kRescale || top1 > mrow[nt][1] + kRescale
+                    || mrow[nt][0] == -INFINITY)) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float mx = h == 0 ? top0 : top1;
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                    float const m_new = fmaxf(mrow[nt][h], mx);
+                    float const alpha = mrow[nt][h] == -INFINITY ? 0.f : exp2_approx(mrow[nt][h] - m_new);
+                    lrow[nt][h] *= alpha;
+                    mrow[nt][h] = m_new;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        o[nt][j][h] *= alpha;
+                        o[nt][j][2 + h] *= alpha;
+                    }
+                }
+            }
             float p[4];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                float const xa = tg ? st[nt][h] * a.scale_log2 : -INFINITY;
-                float const xb = tg8 ? st[nt][2 + h] * a.scale_log2 : -INFINITY;
-                float mx = fmaxf(xa, xb);
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                float const m_new = fmaxf(mrow[nt][h], mx);
-                float const m_use = m_new == -INFINITY ? 0.f : m_new;
-                float const alpha = exp2_approx(mrow[nt][h] - m_use);
-                p[h] = exp2_approx(xa - m_use);
-                p[2 + h] = exp2_approx(xb - m_use);
-                lrow[nt][h] = lrow[nt][h] * alpha + p[h] + p[2 + h];
-                mrow[nt][h] = m_new;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    o[nt][j][h] *= alpha;
-                    o[nt][j][2 + h] *= alpha;
-                }
+                float const use = mrow[nt][h] == -INFINITY ? 0.f : mrow[nt][h];
+                p[h] = exp2_approx(x[h] - use);
+                p[2 + h] = exp2_approx(x[2 + h] - use);
+                lrow[nt][h] += p[h] + p[2 + h];
             }
             float hp[4];
 #pragma unroll
@@ -1035,14 +1051,14 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_attention_kernel(const __g
     if (blockIdx.x >= a.plan.num_shared) {
         pdl_wait();
         pdl_launch_dependents();  // behind the wait: the joining launch reads the plan before its own
-        if (warp >= kSoftWarps) {
+        if (warp >= kOwnWarps) {
             return;
         }
         std::uint32_t const own = a.plan.num_items - a.plan.num_shared;
         std::uint32_t const first = (blockIdx.x - a.plan.num_shared) * a.plan.tasks_per_cta;
         std::uint32_t const left = own - first;
         std::uint32_t const count = left < a.plan.tasks_per_cta ? left : a.plan.tasks_per_cta;
-        for (std::uint32_t t = warp; t < count; t += kSoftWarps) {
+        for (std::uint32_t t = warp; t < count; t += kOwnWarps) {
             kk_prefix_item const item = a.items[a.plan.num_shared + first + t];
             if (item.row_tiles != 0 || item.owner >= a.plan.num_lanes || item.kv_head >= a.kv_heads
                 || item.desc_begin > item.desc_end || item.desc_end > a.plan.num_descs
@@ -1341,7 +1357,7 @@ int kk_prefix_attention_plan(const kk_page_desc* descs, uint32_t num_descs, kk_a
         || (max_items != 0 && items == nullptr)) {
         return KK_EINVAL;
     }
-    *plan = kk_prefix_plan{0, 0, kSoftWarps, num_lanes, num_groups, num_descs, q_heads, kv_heads, 0};
+    *plan = kk_prefix_plan{0, 0, kOwnWarps, num_lanes, num_groups, num_descs, q_heads, kv_heads, 0};
     std::uint32_t const ratio = q_heads / kv_heads;
     auto outside = [&](std::uint32_t offset, std::uint32_t count) {
         return offset > num_descs || count > num_descs - offset;
@@ -1413,7 +1429,7 @@ int kk_prefix_attention_plan(const kk_page_desc* descs, uint32_t num_descs, kk_a
         double const tasks = tasksOf(taskTokensIn(ns));
         double const tokens = static_cast<double>(own_tokens) * kv_heads;
         double const rounds = roundsIn(ns, tasks);
-        return std::fmax(std::ceil(tasks / (rounds * kSoftWarps)),
+        return std::fmax(std::ceil(tasks / (rounds * kOwnWarps)),
             std::ceil(tokens * kOwnTokenNs / std::fmax(1., ns - kOwnNs - kTaskNs)));
     };
     auto sharedBlocksIn = [&](double ns) {
@@ -1484,7 +1500,7 @@ int kk_prefix_attention_plan(const kk_page_desc* descs, uint32_t num_descs, kk_a
         }
         // The shortest items that those blocks take in as many rounds.
         double const longest_task = taskTokensIn(time);
-        double const room = std::floor(roundsIn(time, tasksOf(longest_task))) * blocks * kSoftWarps;
+        double const room = std::floor(roundsIn(time, tasksOf(longest_task))) * blocks * kOwnWarps;
         double tokens = kOwnMinTokens;
         while (tokens < longest_task && tasksOf(tokens) > room) {
             tokens *= 1.125;
@@ -1499,30 +1515,53 @@ int kk_prefix_attention_plan(const kk_page_desc* descs, uint32_t num_descs, kk_a
                 continue;
             }
             std::uint64_t const parts = (len + per_task - 1u) / per_task;
-            std::uint64_t const goal = (len + parts - 1u) / parts;
             ln.item_offset = static_cast<std::uint32_t>(part_rows);
             std::uint32_t begin = ln.desc_offset;
             std::uint64_t held = 0;
-            for (std::uint32_t e = ln.desc_offset; e < end; ++e) {
-                held += 8u * groupsOf(descs[e]);
-                if (held >= goal || e + 1u == end) {
-                    for (std::uint32_t h = 0; h < kv_heads; ++h) {
-                        put(kk_prefix_item{b, h, begin, e + 1u, ln.item_count, 0, 0, 0,
-                            static_cast<std::uint32_t>(part_rows) + h * ratio, 0, 0, ln.query_row, 0});
-                    }
-                    ++ln.item_count;
-                    part_rows += q_heads;
-                    if (part_rows > 0xffffffffull) {
-                        return KK_EINVAL;
-                    }
-                    begin = e + 1u;
-                    held = 0;
+            // Cut i lies at the page boundary nearest to i / parts of the tokens.
+            std::uint64_t seen = 0;
+            auto goal = [&]() {
+                return ln.item_count + 1u < parts ? len * (ln.item_count + 1u) / parts : ~std::uint64_t{0};
+            };
+            auto emit = [&](std::uint32_t to) {
+                for (std::uint32_t h = 0; h < kv_heads; ++h) {
+                    put(kk_prefix_item{b, h, begin, to, ln.item_count, 0, 0, 0,
+                        static_cast<std::uint32_t>(part_rows) + h * ratio, 0, 0, ln.query_row, 0});
                 }
+                ++ln.item_count;
+                part_rows += q_heads;
+                begin = to;
+                held = 0;
+            };
+            for (std::uint32_t e = ln.desc_offset; e < end; ++e) {
+                std::uint64_t const more = 8u * groupsOf(descs[e]);
+                if (held != 0 && seen + more > goal() && (seen >= goal() || seen + more - goal() > goal() - seen)) {
+                    emit(e);
+                }
+                held += more;
+                seen += more;
+                if (seen >= goal()) {
+                    emit(e + 1u);
+                }
+            }
+            if (held != 0) {
+                emit(end);
+            } else {
+                // Pages without tokens behind the last cut belong to the last items.
+                for (std::uint32_t h = 0; begin != end && h < kv_heads; ++h) {
+                    std::uint32_t const last = count - kv_heads + h;
+                    if (last < max_items) {
+                        items[last].desc_end = end;
+                    }
+                }
+            }
+            if (part_rows > 0xffffffffull) {
+                return KK_EINVAL;
             }
         }
         std::uint32_t const tasks = count - plan->num_shared;
         std::uint32_t const per_cta = (tasks + blocks - 1u) / blocks;
-        plan->tasks_per_cta = per_cta < kSoftWarps ? kSoftWarps : per_cta;
+        plan->tasks_per_cta = per_cta < kOwnWarps ? kOwnWarps : per_cta;
     }
     plan->num_items = count;
     plan->part_rows = part_rows;
