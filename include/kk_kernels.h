@@ -295,8 +295,9 @@ typedef struct kk_prefix_attn_desc {
 } kk_prefix_attn_desc;
 /* A lane that has no tokens at all gets zeros. Descriptors outside their pool
  * or over their page contribute nothing and are reported by kk_device_status,
- * as are items that do not fit the plan. query and output are 16-byte aligned,
- * strides multiples of 8. */
+ * as are items that do not fit the plan. query, output and workspace are
+ * 16-byte aligned, the plan's arrays 4-byte, strides multiples of 8. Two lanes
+ * must not name the same query row. */
 KK_KAPI int kk_prefix_attention(const kk_prefix_attn_desc* desc, void* stream);
 
 /* ---- K2: batched KV append / copy-on-write -----------------------------------
@@ -327,7 +328,7 @@ KK_KAPI int kk_kv_copy_tokens(const kk_kv_pools* pools, uint32_t layer_begin,
  * table, skips the row too and is reported by kk_device_status. Two active
  * rows of one call must not name the same (slot, token).
  * head_dim % 8 == 0, rotary_dim % 16 == 0, rotary_dim <= min(head_dim, 256);
- * pointers 16-byte aligned (cos_sin: 8), strides multiples of 8 and not below
+ * pointers 16-byte aligned (cos_sin: 8, slots and positions: 4), strides multiples of 8 and not below
  * the row they step over. query_out may be query itself (same stride). */
 typedef struct kk_kv_append_desc {
     kk_kv_pools pools;
@@ -494,9 +495,10 @@ KK_KAPI int kk_gemm(const kk_gemm_desc* desc, void* stream);
  * Strides are in elements; rows may start at any multiple of 4 bytes. vocab is
  * at most 400,000 where a history or biases are given, 10 million otherwise.
  * Ids outside the vocabulary are ignored. Offsets that decrease or pass their
- * array, bias ids that descend within a row and mask rows outside the masks are
- * reported by kk_device_status; the row's history or biases are then left
- * out, respectively the row is masked entirely. */
+ * array and mask rows outside the masks are reported by kk_device_status; the
+ * row's history or biases are then left out, respectively the row is masked
+ * entirely. Bias ids that descend within a row are reported too; what that row
+ * gets of its biases is not specified. Arrays are 4-byte aligned. */
 #define KK_NO_TOKEN 0xffffffffu
 #define KK_NO_MASK 0xffffffffu
 typedef struct kk_logits_desc {

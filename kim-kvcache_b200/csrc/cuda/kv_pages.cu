@@ -463,7 +463,8 @@ int kk_kv_append_rope(const kk_kv_append_desc* d, void* stream)
     if (d->rows == 0) {
         return 0;
     }
-    if (d->slots == nullptr || misaligned(d->key, d->key_stride, kv_row)
+    auto odd = [](void const* p) { return (reinterpret_cast<std::uintptr_t>(p) & 3u) != 0; };
+    if (d->slots == nullptr || odd(d->slots) || misaligned(d->key, d->key_stride, kv_row)
         || misaligned(d->value, d->value_stride, kv_row)
         || (d->q_heads != 0
             && (misaligned(d->query, d->query_stride, q_row) || misaligned(d->query_out, d->query_out_stride, q_row)
@@ -472,7 +473,7 @@ int kk_kv_append_rope(const kk_kv_append_desc* d, void* stream)
     }
     AppendArgs a{};
     if (d->rotary_dim != 0) {
-        if (d->positions == nullptr || (reinterpret_cast<std::uintptr_t>(d->cos_sin) & 7u) != 0
+        if (d->positions == nullptr || odd(d->positions) || (reinterpret_cast<std::uintptr_t>(d->cos_sin) & 7u) != 0
             || (d->cos_sin != nullptr && d->table_positions == 0)
             || (d->cos_sin == nullptr && !(d->theta >= 1.f && std::isfinite(d->theta)))) {
             return KK_EINVAL;
@@ -512,7 +513,7 @@ int kk_kv_append_rope(const kk_kv_append_desc* d, void* stream)
     a.key_stride = d->key_stride;
     a.value_stride = d->value_stride;
     a.query_out_stride = d->query_out_stride;
-    unsigned const grid = (d->rows + a.rows_per_cta - 1u) / a.rows_per_cta;
+    unsigned const grid = (d->rows - 1u) / a.rows_per_cta + 1u;
     return static_cast<int>(launch(kv_append_rope_kernel, dim3(grid), dim3(kAppendThreads), 0,
         static_cast<cudaStream_t>(stream), 1, a));
 }

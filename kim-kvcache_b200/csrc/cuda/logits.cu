@@ -554,6 +554,16 @@ extern "C" int kk_logits_process(const kk_logits_desc* d, void* stream)
         || odd(d->tokens)) {
         return KK_EINVAL;
     }
+    for (void const* array : {static_cast<void const*>(d->history), static_cast<void const*>(d->history_offsets),
+             static_cast<void const*>(d->prompt_counts), static_cast<void const*>(d->repetition),
+             static_cast<void const*>(d->presence), static_cast<void const*>(d->frequency),
+             static_cast<void const*>(d->bias_tokens), static_cast<void const*>(d->bias_values),
+             static_cast<void const*>(d->bias_offsets), static_cast<void const*>(d->mask),
+             static_cast<void const*>(d->mask_rows)}) {
+        if (odd(array)) {
+            return KK_EINVAL;
+        }
+    }
     LogitsArgs a{};
     a.d = *d;
     bool const penalties = d->repetition != nullptr || d->presence != nullptr || d->frequency != nullptr;

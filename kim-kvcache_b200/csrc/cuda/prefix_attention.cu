@@ -1091,6 +1091,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_attention_kernel(const __g
         sh->abort = 0;
         fence_barrier_init();
     }
+    // All of TMEM, before the wait for what ran before: the block's shared memory
+    // leaves room on the SM for none of the other kernels that use TMEM.
     if (warp == kIssuerWarp) {
         tmem_alloc(&sh->tmem, kTmemCols);
         tmem_relinquish();
@@ -1153,7 +1155,12 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(const __grid_
         return;
     }
     // The plan is older than the launch that writes the partials: it is read
-    // before that one has ended.
+    // before that one has ended. (That one began to let this one start behind its
+    // own wait. Without items there is none, and what runs before may be the copy of
+    // the plan.)
+    if (a.plan.num_items == 0) {
+        pdl_wait();
+    }
     std::uint32_t const qh = t / 32u % q_heads;
     std::uint32_t const chunk = t % 16u;
     kk_attn_lane const ln = a.lanes[lane];
@@ -1588,11 +1595,11 @@ int kk_prefix_attention(const kk_prefix_attn_desc* d, void* stream)
         return 0;
     }
     std::uint64_t const q_row = std::uint64_t(d->q_heads) * kHeadDim;
-    if (d->lanes == nullptr || misaligned(d->query) || misaligned(d->output) || d->query_stride % 8 != 0
+    auto odd = [](void const* p) { return (reinterpret_cast<std::uintptr_t>(p) & 3u) != 0; };
+    if (d->lanes == nullptr || odd(d->lanes) || odd(d->groups) || odd(d->items) || odd(d->descs) || misaligned(d->query) || misaligned(d->output) || d->query_stride % 8 != 0
         || d->output_stride % 8 != 0 || d->query_stride < q_row || d->output_stride < q_row
         || (d->plan.num_groups != 0 && d->groups == nullptr)
         || (d->plan.num_items != 0 && (d->items == nullptr || d->descs == nullptr))
-        || (d->plan.num_descs != 0 && (reinterpret_cast<std::uintptr_t>(d->descs) & 3u) != 0)
         || (d->plan.part_rows != 0
             && (misaligned(d->workspace)
                 || d->workspace_bytes < kk_prefix_attention_workspace_bytes(&d->plan)))) {
@@ -1662,10 +1669,10 @@ int kk_prefix_attention(const kk_prefix_attn_desc* d, void* stream)
             return rc;
         }
     }
-    // The joining launch is always a programmatic dependent of the first: its
-    // blocks are set up while the last items run, and wait for their end.
+    // The joining launch is always a programmatic dependent of the first, if there is
+    // one: its blocks are set up while the last items run, and wait for their end.
     bool const pdl = g_pdl_enabled;
-    g_pdl_enabled = true;
+    g_pdl_enabled = pdl || d->plan.num_items != 0;
     int const rc = static_cast<int>(launch(prefix_join_kernel,
         dim3(static_cast<unsigned>((threads + kJoinThreads - 1u) / kJoinThreads)), dim3(kJoinThreads), 0, s, 1, a));
     g_pdl_enabled = pdl;

@@ -39,6 +39,7 @@ def valid_desc(kk):
     dict(query=None), dict(query_out=None), dict(key=None), dict(value=None), dict(key=(1 << 16) + 2),
     dict(query=(1 << 16) + 8), dict(value_stride=132), dict(key_stride=120), dict(query_stride=248),
     dict(query_out_stride=248), dict(query_stride=264), dict(cos_sin=1 << 14),  # no table_positions
+    dict(slots=(1 << 12) + 2), dict(positions=(1 << 12) + 1),
     dict(cos_sin=(1 << 14) + 4, table_positions=9), dict(q_heads=1 << 20),
     dict(pools=(1 << 20, 1 << 21, 8, 4, 2, 2, 60, 8)), dict(pools=(1 << 20, 1 << 21, 8, 4, 0, 2, 64, 8)),
     dict(pools=(1 << 20, 1 << 21, 8, 4, 2, 2, 64, 24)), dict(pools=((1 << 20) + 4, 1 << 21, 8, 4, 2, 2, 64, 8)),

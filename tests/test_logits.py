@@ -32,6 +32,10 @@ def valid_desc(kk):
     dict(frequency=16), dict(repetition=16, history_offsets=16, history_size=4),
     dict(bias_offsets=16, bias_size=3), dict(bias_offsets=16, bias_size=3, bias_tokens=16),
     dict(mask=16, mask_stride=3, num_masks=2), dict(vocab=(1 << 30) + 1, logits_stride=1 << 31, out_stride=1 << 31),
+    dict(repetition=16, history_offsets=18, history=16, history_size=4), dict(repetition=17, history_offsets=16),
+    dict(repetition=16, history_offsets=16, history=18, history_size=4), dict(bias_offsets=18),
+    dict(bias_offsets=16, bias_tokens=18, bias_values=16, bias_size=1), dict(mask=18, mask_stride=4, num_masks=2),
+    dict(mask=16, mask_stride=4, num_masks=2, mask_rows=17),
     dict(vocab=500000, logits_stride=500000, out_stride=500000, bias_offsets=16),
     dict(vocab=20000000, logits_stride=20000000, out_stride=20000000, mask=16, mask_stride=625000, num_masks=1),
 ], ids=str)

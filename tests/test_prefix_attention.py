@@ -234,6 +234,7 @@ def valid_desc(kk):
 @pytest.mark.parametrize("change", [
     dict(layer=2), dict(q_heads=16), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
     dict(scale=float("inf")), dict(descs=None), dict(lanes=None), dict(groups=None), dict(items=None),
+    dict(descs=(1 << 12) + 2), dict(lanes=(1 << 12) + 1), dict(groups=(1 << 12) + 2), dict(items=(1 << 12) + 2),
     dict(query=None), dict(output=None), dict(query=(1 << 16) + 8), dict(output=(1 << 16) + 2),
     dict(query_stride=2044), dict(output_stride=2040), dict(workspace=None), dict(workspace=(1 << 16) + 8),
     dict(workspace_bytes=263999), dict(pools=(1 << 20, 1 << 21, 8, 4, 2, 4, 128, 8)),
@@ -304,7 +305,7 @@ class Setup:
 
     def reference(self, layer, b):
         """64-bit result of lane b, and the size of the errors that FP32 sums leave in it."""
-        parts = [(self.extent if k else self.micro)[s, layer, :, :n] for s, _, n, k in self.tables[b]]
+        parts = [(self.extent if k else self.micro)[s, layer, :, :n] for s, _, n, k in self.tables[b] if n]
         if not parts:
             return torch.zeros(self.hq, 64, dtype=torch.float64, device="cuda"), 0.0
         k, v = torch.cat(parts, 1).double()
@@ -392,6 +393,26 @@ def test_prefix_many_groups_and_lanes_without_one(kk):
     assert alone.plan.num_shared == 0
     alone.run()
     alone.check()
+
+
+@gpu_test
+def test_prefix_pages_without_tokens(kk):
+    """Tables with pages that hold nothing yet, more in a row than a warp looks at once, at the start, inside and
+    at the end; lanes and prefixes made of nothing else."""
+    pages = Pages(random.Random(17))
+
+    def empty(n):
+        return [(pages.take(0), 0, 0, 0) for _ in range(n)]
+
+    shared = empty(1) + pages.table(100) + empty(70) + pages.table(200, 100) + empty(33)
+    tables = [shared + tail for tail in (empty(40) + pages.table(30) + empty(1), [], empty(3), pages.table(5) + empty(65))]
+    nothing = empty(2)
+    tables += [nothing + pages.table(9), list(nothing), empty(1), []]
+    for sms in (1, 148):
+        s = Setup(kk, tables, pages, 8, 2, 18, sms)
+        assert s.ng == 1
+        s.run()
+        s.check()
 
 
 @gpu_test
