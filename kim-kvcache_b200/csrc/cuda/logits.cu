@@ -6,29 +6,35 @@
 // with one contiguous slice per CTA the first one had half of the history). A CTA
 //  1. counts, in shared memory, what of the row's history is its own (every CTA
 //     reads the whole history) and marks the tokens, a bit each;
-//  2. lists the marked tokens and replaces their counts by their penalised logits;
-//  3. adds the biases to those, or to the plain logits;
-//  4. streams its logits, 256 tokens a warp at a time (rows that start on odd
-//     addresses included), takes the marked ones from shared memory, applies
-//     the mask and keeps the highest; the cluster's winners meet in its first
-//     CTA.
+//  2. lists the marked tokens, works out their penalised logits and replaces their
+//     counts by their places in the list;
+//  3. adds the biases to those, or lists the plain logits with their biases;
+//  4. streams its logits, 256 tokens a warp at a time, takes the marked ones from
+//     the list, applies the mask and keeps the highest; the cluster's winners meet
+//     in its first CTA.
 // Few tokens of a vocabulary are ever penalised, but few warps of the stream
-// meet none, so step 4 computes nothing for them. Counts are integers and a
-// replaced logit has one writer, so the order of threads changes nothing.
+// meet none, so step 4 computes nothing for them. Counts are integers and a logit
+// has one owner, so the order of threads changes nothing. Counts have 16 bits,
+// which lets four CTAs share an SM: what bounds the kernel is the chain of steps
+// of a CTA. A row with more than 65,535 tokens of history is taken in two halves
+// of the CTA's places, with 32 bits each; more marked tokens than the list holds
+// are taken 2,048 places at a time.
 //
-// HBM bounds it: 4 bytes read and 4 written per logit. The CTA's logits are
+// HBM is the floor: 4 bytes read and 4 written per logit. The CTA's logits are
 // asked into L2 at the start, so that DRAM works while the history is counted.
 // Measured on 256 rows of 128,000 logits with about 10,000 tokens of history
-// each (262 MB, 40 us at the measured copy rate): 130 us; 132 us
-// with the penalties inside the stream (82 instructions a logit); 150 us with
-// contiguous slices and a second pass over the history in place of the list;
-// 200 us with each history read once and counted through distributed shared
-// memory.
+// each (262 MB, 40 us at the measured copy rate): 106 us. 130 us with a 32-bit
+// word per place (three CTAs per SM); 132 us with the marked tokens of a warp's
+// block spread over its lanes there, in place of steps 2 and 3 (twice the
+// instructions); 150 us with contiguous slices and a second pass over the
+// history; 157 us with clusters of 16; 200 us with each history read once and
+// counted through distributed shared memory.
 #include "../../../include/kk_kernels.h"
 #include "kernels_internal.h"
 #include "launch.cuh"
 
 #include <atomic>
+#include <type_traits>
 
 namespace kk {
 
@@ -41,20 +47,23 @@ constexpr std::uint32_t kWarps = kThreads / 32;
 constexpr std::uint32_t kMaxCluster = 8;
 constexpr std::uint32_t kBlock = 256;          // consecutive tokens of one CTA
 constexpr std::uint32_t kQuads = 2;            // 16-byte history loads in flight per thread
-constexpr std::uint32_t kListed = 2048;        // marked tokens listed at most; others are taken bit by bit
-constexpr std::uint32_t kGather = 2;           // listed tokens per thread at a time
+constexpr std::uint32_t kMaxCounted = 65535;   // history of a row that 16-bit counts hold
+constexpr std::uint32_t kMaxWordsVocab = 400000;  // with a history or biases
+constexpr std::uint32_t kMaxVocab = 10000000;     // with a mask
 constexpr std::uint32_t kMaxSharedBytes = 222u * 1024u;
+constexpr std::uint32_t kListed = 2048;        // listed tokens
+constexpr std::uint32_t kGather = 2;           // of them per thread at a time
+constexpr std::uint32_t kFewBlocks = kListed / kBlock;  // whose tokens the list holds in any case
 
 struct LogitsArgs {
     kk_logits_desc d;
     std::uint32_t cluster_log2;  // CTAs per row
-    // Places in shared memory, in 32-bit words; a place of a token is its
-    // number among the CTA's own (the first `capacity`), or capacity + token
-    // for the up to three tokens before the row's first 16-byte step.
-    std::uint32_t capacity;
-    std::uint32_t touched_at;    // a bit per place, set: the word is the token's new logit
+    std::uint32_t capacity;      // places (a token's number among the CTA's own) of a CTA, whole blocks, an even number
+    // In shared memory, in 32-bit words; counts, 16 bits a place, come first.
+    std::uint32_t touched_at;    // a bit per place, set: in the history or biased
+    std::uint32_t value_at;      // logits of listed tokens
+    std::uint32_t list_at;       // and their places, 16 bits each
     std::uint32_t mask_at;       // a bit per place, set: allowed
-    std::uint32_t list_at;       // 16-bit places
 };
 
 __device__ __forceinline__ void report(unsigned int code) { atomicCAS(&g_logits_status, kErrNone, code); }
@@ -69,9 +78,13 @@ __device__ __forceinline__ void cluster_wait()
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-__device__ __forceinline__ void st_cluster_u64(std::uint32_t addr, std::uint64_t v)
+// A store into another CTA's shared memory that its barrier counts: neither side has
+// to order it behind the stores of the logits (a cluster barrier would).
+__device__ __forceinline__ void st_cluster_u64(std::uint32_t addr, std::uint64_t v, std::uint32_t bar)
 {
-    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.u64 [%0], %1, [%2];"
+                 ::"r"(addr), "l"(v), "r"(bar)
+                 : "memory");
 }
 
 // A read-only load issued where it stands in the program.
@@ -97,39 +110,37 @@ __device__ __forceinline__ std::uint64_t candidate(float x, std::uint32_t id)
 __global__ void __launch_bounds__(kThreads, 4) logits_process_kernel(const __grid_constant__ LogitsArgs a)
 {
     extern __shared__ __align__(16) std::uint32_t s_words[];
+    __shared__ std::uint32_t s_listed;
     __shared__ std::uint64_t s_best[kWarps];
     __shared__ std::uint64_t s_cluster[kMaxCluster];
-    __shared__ std::uint32_t s_listed;
+    __shared__ std::uint64_t s_winners;  // barrier: the other CTAs' winners are here
     pdl_launch_dependents();
     pdl_wait();
     kk_logits_desc const& d = a.d;
     std::uint32_t const tid = threadIdx.x;
+    std::uint32_t const lane = tid % 32u;
+    std::uint32_t const warp = tid / 32u;
     std::uint32_t const lc = a.cluster_log2;
     std::uint32_t const rank = blockIdx.x & ((1u << lc) - 1u);
     std::uint32_t const row = blockIdx.x >> lc;
     std::uint32_t const vocab = d.vocab;
-    float const* const in = d.logits + row * d.logits_stride;
-    float* const out = d.out != nullptr ? d.out + row * d.out_stride : nullptr;
-    bool const same_phase = out == nullptr
-        || ((reinterpret_cast<std::uintptr_t>(out) ^ reinterpret_cast<std::uintptr_t>(in)) & 15u) == 0;
-    // Tokens before the first 16-byte step; the first CTA's.
-    std::uint32_t head = (4u - static_cast<std::uint32_t>(reinterpret_cast<std::uintptr_t>(in) >> 2)) & 3u;
-    head = head < vocab ? head : vocab;
-    std::uint32_t const body = vocab - head;
-    std::uint32_t const all_blocks = (body + kBlock - 1u) / kBlock;
+    // Blocks start on a 16-byte boundary: token v stands at u = v + shift of them.
+    float const* in = d.logits + row * d.logits_stride;
+    std::uint32_t const shift = static_cast<std::uint32_t>(reinterpret_cast<std::uintptr_t>(in) >> 2) & 3u;
+    in -= shift;
+    float* const out = d.out != nullptr ? d.out + row * d.out_stride - shift : nullptr;
+    bool const vector_out = (reinterpret_cast<std::uintptr_t>(out) & 15u) == 0;
+    std::uint32_t const end = vocab + shift;
+    std::uint32_t const all_blocks = (end + kBlock - 1u) / kBlock;
     std::uint32_t const blocks = all_blocks > rank ? ((all_blocks - 1u - rank) >> lc) + 1u : 0u;
-    // Place <-> token, behind the head.
-    auto token_of = [&](std::uint32_t at) {
-        return head + ((((at / kBlock) << lc) + rank) * kBlock) + at % kBlock;
-    };
+    auto first_of = [&](std::uint32_t block) { return ((block << lc) + rank) * kBlock; };  // a block's first u
     std::uint32_t const owner_mask = ((1u << lc) - 1u) * kBlock;
     std::uint32_t const owner = rank * kBlock;
-    auto owned = [&](std::uint32_t v) { return v - head < body && ((v - head) & owner_mask) == owner; };
+    auto owned = [&](std::uint32_t v) { return ((v + shift) & owner_mask) == owner && v < vocab; };
     auto place_of = [&](std::uint32_t v) {
-        std::uint32_t const u = v - head;
+        std::uint32_t const u = v + shift;
         return ((u / kBlock) >> lc) * kBlock + u % kBlock;
     };
-    auto in_head = [&](std::uint32_t v) { return v < head && rank == 0; };
 
     // ---- everything that can be asked for at once
     float rep = 1.f, pres = 0.f, freq = 0.f;
@@ -150,20 +161,26 @@ __global__ void __launch_bounds__(kThreads, 4) logits_process_kernel(const __gri
         mask_row = ldg_u32_now(d.mask_rows + row);
     }
     for (std::uint32_t i = tid; i < blocks; i += kThreads) {
-        std::uint32_t const v = token_of(i * kBlock);
-        std::uint32_t const n = (vocab - v < kBlock ? vocab - v : kBlock) / 4u;
-        if (n != 0) {
-            l2_prefetch_bulk(in + v, n * 16u);
+        std::uint32_t u = first_of(i);
+        std::uint32_t const stop = (u + kBlock < end ? u + kBlock : end) & ~3u;
+        u = u < shift ? 4u : u;  // whole steps only: nothing before or behind the row is touched
+        if (u < stop) {
+            l2_prefetch_bulk(in + u, (stop - u) * 4u);
         }
     }
     std::uint32_t* const s_touched = s_words + a.touched_at;
-    if (a.touched_at != 0) {  // the call has a history or biases
-        if (d.history_offsets != nullptr) {
-            for (std::uint32_t i = tid; i <= a.capacity / 4u; i += kThreads) {
-                reinterpret_cast<uint4*>(s_words)[i] = make_uint4(0, 0, 0, 0);
-            }
+    float* const s_value = reinterpret_cast<float*>(s_words + a.value_at);
+    std::uint16_t* const s_list = reinterpret_cast<std::uint16_t*>(s_words + a.list_at);
+    auto clear_counts = [&]() {
+        for (std::uint32_t i = tid; i < a.capacity / 8u; i += kThreads) {
+            reinterpret_cast<uint4*>(s_words)[i] = make_uint4(0, 0, 0, 0);
         }
-        for (std::uint32_t i = tid; i <= a.capacity / 32u; i += kThreads) {
+    };
+    if (d.history_offsets != nullptr) {
+        clear_counts();
+    }
+    if (a.value_at != 0) {  // the call has a history or biases
+        for (std::uint32_t i = tid; i < a.capacity / 32u; i += kThreads) {
             s_touched[i] = 0;
         }
         if (tid == 0) {
@@ -195,7 +212,7 @@ __global__ void __launch_bounds__(kThreads, 4) logits_process_kernel(const __gri
         report(kErrBadArgument);
     }
     bool const penal = h1 > h0;
-    bool const use_words = penal || b1 > b0;
+    bool const biased = b1 > b0;
     // The thread's first 16-byte pieces of the history.
     std::uint32_t const* const text = d.history + h0;
     std::uint32_t const len = h1 - h0;
@@ -219,174 +236,36 @@ __global__ void __launch_bounds__(kThreads, 4) logits_process_kernel(const __gri
     float bias_value = 0.f, bias_logit = 0.f;
     auto load_bias = [&](std::uint32_t i) {
         bias_token = d.bias_tokens[i];
-        bias_next = i + 1 < b1 ? d.bias_tokens[i + 1] : 0xffffffffu;
+        bias_next = i + 1u < b1 ? d.bias_tokens[i + 1u] : 0xffffffffu;
         bias_value = d.bias_values[i];
-        bias_logit = owned(bias_token) || in_head(bias_token) ? in[bias_token] : 0.f;
+        bias_logit = owned(bias_token) ? in[bias_token + shift] : 0.f;
     };
     if (b0 + tid < b1) {
         load_bias(b0 + tid);
     }
+    std::uint32_t* const s_mask = s_words + a.mask_at;
+    if (mask != nullptr) {
+        // Brought to the places' order; words behind the vocabulary are never asked for.
+        std::uint32_t const words = (vocab + 31u) / 32u;
+        for (std::uint32_t i = tid; i < blocks * (kBlock / 32u); i += kThreads) {
+            std::uint32_t const w = first_of(i / (kBlock / 32u)) / 32u + i % (kBlock / 32u);
+            std::uint32_t const low = shift != 0 && w - 1u < words ? __ldg(mask + w - 1u) : 0u;
+            s_mask[i] = __funnelshift_l(low, w < words ? __ldg(mask + w) : 0u, shift);
+        }
+    }
     // Before a CTA writes into another one's shared memory, all of the cluster
     // have started: they say so here and ask at the end.
     if (lc != 0 && d.tokens != nullptr) {
-        cluster_arrive();
-    }
-
-    std::uint32_t* const s_mask = s_words + a.mask_at;
-    std::uint16_t* const s_list = reinterpret_cast<std::uint16_t*>(s_words + a.list_at);
-    if (mask != nullptr) {
-        // Brought to the places' order; bits behind the vocabulary are never asked for.
-        std::uint32_t const last = (vocab - 1u) / 32u;
-        for (std::uint32_t i = tid; i < blocks * (kBlock / 32u); i += kThreads) {
-            std::uint32_t const v = token_of(i * 32u);
-            std::uint32_t const w = v / 32u < last ? v / 32u : last;
-            s_mask[i] = __funnelshift_r(__ldg(mask + w), __ldg(mask + (w < last ? w + 1u : last)), v & 31u);
+        if (rank == 0 && tid == 0) {
+            mbar_init(&s_winners, 1);
+            fence_barrier_init();
+            mbar_arrive_expect_tx(&s_winners, ((1u << lc) - 1u) * 8u);
         }
+        __syncwarp();
+        cluster_arrive();
     }
     __syncthreads();
 
-    // ---- the history and the biases
-    if (penal) {
-        auto count = [&](std::uint32_t at, std::uint32_t i) {
-            atomicOr(&s_touched[at / 32u], 1u << (at % 32u));
-            if (i >= prompt) {
-                atomicAdd(&s_words[at], 1u);
-            }
-        };
-        for (std::uint32_t q0 = tid; q0 < quads; q0 += kThreads * kQuads) {
-            uint4 now[kQuads];
-#pragma unroll
-            for (std::uint32_t k = 0; k < kQuads; ++k) {
-                now[k] = ahead[k];
-            }
-            load_quads(q0 + kThreads * kQuads);
-#pragma unroll
-            for (std::uint32_t k = 0; k < kQuads; ++k) {
-                std::uint32_t const i = from + (q0 + k * kThreads) * 4u;
-                uint4 const t = now[k];
-                std::uint32_t const v[4] = {t.x, t.y, t.z, t.w};
-#pragma unroll
-                for (std::uint32_t e = 0; e < 4u; ++e) {
-                    if (owned(v[e])) {
-                        count(place_of(v[e]), i + e);
-                    }
-                }
-                if (head != 0) {
-#pragma unroll
-                    for (std::uint32_t e = 0; e < 4u; ++e) {
-                        if (in_head(v[e])) {
-                            count(a.capacity + v[e], i + e);
-                        }
-                    }
-                }
-            }
-        }
-        std::uint32_t const edge = tid < from ? tid : from + quads * 4u + (tid - from);
-        if (edge < len && tid < from + 3u) {
-            std::uint32_t const v = text[edge];
-            if (owned(v)) {
-                count(place_of(v), edge);
-            } else if (in_head(v)) {
-                count(a.capacity + v, edge);
-            }
-        }
-        __syncthreads();
-        auto logit_at = [&](std::uint32_t at) { return in[at < a.capacity ? token_of(at) : at - a.capacity]; };
-        auto penalise = [&](std::uint32_t at, float x) {
-            std::uint32_t const n = s_words[at];
-            x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
-            if (n != 0) {
-                x = __fsub_rn(x, __fmul_rn(freq, static_cast<float>(n)));
-                x = __fsub_rn(x, pres);
-            }
-            s_words[at] = __float_as_uint(x);
-        };
-        // Marked tokens lie in clumps: they are spread over the threads by a list.
-        std::uint32_t const words = blocks * (kBlock / 32u);
-        for (std::uint32_t i0 = 0; i0 <= words; i0 += kThreads) {
-            std::uint32_t const i = i0 + tid;
-            std::uint32_t const w = i < words ? i : a.capacity / 32u;  // the head's word stands behind all blocks
-            std::uint32_t bits = i <= words ? s_touched[w] : 0u;
-            std::uint32_t const own = __popc(bits);
-            std::uint32_t upto = own;
-#pragma unroll
-            for (std::uint32_t o = 1; o < 32u; o *= 2u) {
-                std::uint32_t const x = __shfl_up_sync(0xffffffffu, upto, o);
-                upto += tid % 32u >= o ? x : 0u;
-            }
-            std::uint32_t base = 0;
-            if (tid % 32u == 31u && upto != 0) {
-                base = atomicAdd(&s_listed, upto);
-            }
-            std::uint32_t n = __shfl_sync(0xffffffffu, base, 31) + upto - own;
-            auto list = [&](std::uint32_t at, std::uint32_t place) {
-                if (place < kListed) {
-                    s_list[place] = static_cast<std::uint16_t>(at);
-                } else {
-                    penalise(at, logit_at(at));
-                }
-            };
-            // A word with many marks is taken by the whole warp, a lane a bit.
-            for (std::uint32_t full = __ballot_sync(0xffffffffu, own > 4u); full != 0; full &= full - 1u) {
-                std::uint32_t const from_lane = __ffs(full) - 1u;
-                std::uint32_t const word = __shfl_sync(0xffffffffu, bits, from_lane);
-                std::uint32_t const first = __shfl_sync(0xffffffffu, n, from_lane);
-                std::uint32_t const at = __shfl_sync(0xffffffffu, w, from_lane) * 32u + tid % 32u;
-                if ((word >> (tid % 32u) & 1u) != 0) {
-                    list(at, first + __popc(word & ((1u << (tid % 32u)) - 1u)));
-                }
-            }
-            // Straight-line, as above: loops of divergent length cost three times as much.
-#pragma unroll
-            for (std::uint32_t e = 0; e < 4u; ++e) {
-                if (own <= 4u && bits != 0) {
-                    list(w * 32u + __ffs(bits) - 1u, n++);
-                    bits &= bits - 1u;
-                }
-            }
-        }
-        __syncthreads();
-        std::uint32_t const listed = s_listed < kListed ? s_listed : kListed;
-        for (std::uint32_t i0 = tid; i0 < listed; i0 += kThreads * kGather) {
-            std::uint32_t at[kGather];
-            float x[kGather];
-#pragma unroll
-            for (std::uint32_t k = 0; k < kGather; ++k) {
-                std::uint32_t const i = i0 + k * kThreads;
-                at[k] = i < listed ? s_list[i] : 0u;
-                x[k] = i < listed ? logit_at(at[k]) : 0.f;
-            }
-#pragma unroll
-            for (std::uint32_t k = 0; k < kGather; ++k) {
-                if (i0 + k * kThreads < listed) {
-                    penalise(at[k], x[k]);
-                }
-            }
-        }
-        __syncthreads();
-    }
-    for (std::uint32_t i = b0 + tid; i < b1; i += kThreads) {
-        if (i != b0 + tid) {
-            load_bias(i);
-        }
-        std::uint32_t const v = bias_token;
-        if (bias_next < v) {
-            report(kErrBadArgument);
-        }
-        bool const low = in_head(v);
-        if ((low || owned(v)) && bias_next != v) {
-            std::uint32_t const at = low ? a.capacity + v : place_of(v);
-            bool const replaced = (s_touched[at / 32u] >> (at % 32u) & 1u) != 0;
-            s_words[at] = __float_as_uint(
-                __fadd_rn(replaced ? __uint_as_float(s_words[at]) : bias_logit, bias_value));
-            atomicOr(&s_touched[at / 32u], 1u << (at % 32u));
-        }
-    }
-    if (b1 > b0) {
-        __syncthreads();
-    }
-
-    // ---- the logits
     // The highest logit so far and where: a thread meets its steps of four tokens in
     // ascending order, so a strict comparison keeps the lowest of equal ones; NaN
     // and -inf never pass it.
@@ -394,83 +273,290 @@ __global__ void __launch_bounds__(kThreads, 4) logits_process_kernel(const __gri
     std::uint32_t top_id = 0;
     auto bits_of = [&](std::uint32_t const* bits, std::uint32_t at) { return bits[at / 32u] >> (at % 32u); };
     bool const masked = mask != nullptr || blocked;
-    std::uint64_t best = 0;  // of the tokens outside whole blocks
-    auto one = [&](std::uint32_t at, std::uint32_t v) {
-        bool const low = at >= a.capacity;
-        bool const allowed = !blocked
-            && (mask == nullptr || ((low ? mask[0] >> v : bits_of(s_mask, at)) & 1u) != 0);
-        float x = use_words && (bits_of(s_touched, at) & 1u) != 0 ? __uint_as_float(s_words[at]) : in[v];
-        x = allowed ? x : -INFINITY;
-        std::uint64_t const c = candidate(x, v);
-        best = c > best ? c : best;
-        if (out != nullptr) {
-            out[v] = x;
-        }
-    };
-    if (rank == 0 && tid < head) {
-        one(a.capacity + tid, tid);
-    }
-    // A warp takes a block of 256 tokens: two steps of four for every thread. The
-    // places of consecutive blocks of a warp lie kWarps blocks apart, their
-    // tokens that times the cluster's size.
-    std::uint32_t const lane4 = (tid % 32u) * 4u;
-    std::uint32_t const whole_blocks = blocks != 0 && token_of((blocks - 1u) * kBlock) + kBlock > vocab ? blocks - 1u : blocks;
-    {
-        std::uint32_t at = tid / 32u * kBlock + lane4;
-        std::uint32_t v = head + ((tid / 32u << lc) + rank) * kBlock + lane4;
-        std::uint32_t const stride = (kWarps * kBlock) << lc;
-        bool const vector_out = out != nullptr && same_phase;
-        for (std::uint32_t block = tid / 32u; block < whole_blocks; block += kWarps, at += kWarps * kBlock, v += stride) {
-            float4 x[2] = {*reinterpret_cast<float4 const*>(in + v), *reinterpret_cast<float4 const*>(in + v + 128u)};
-            if (use_words) {
+    bool const wide = len > kMaxCounted;
+    std::uint32_t const span = wide ? a.capacity / 2u : a.capacity;  // places counted at a time
+    for (std::uint32_t place0 = 0; place0 == 0 || (wide && place0 < a.capacity); place0 += span) {
+        // ---- the history
+        if (penal) {
+            if (place0 != 0) {
+                __syncthreads();
+                clear_counts();
+                if (tid == 0) {
+                    s_listed = 0;
+                }
+                load_quads(tid);
+                __syncthreads();
+            }
+            auto scan = [&](auto narrow) {
+                auto count = [&](std::uint32_t v, std::uint32_t i) {
+                    if (owned(v)) {
+                        std::uint32_t const at = place_of(v);
+                        atomicOr(&s_touched[at / 32u], 1u << (at % 32u));
+                        if (i >= prompt) {
+                            if (narrow) {
+                                atomicAdd(&s_words[at / 2u], 1u << (at % 2u * 16u));
+                            } else if (at - place0 < span) {
+                                atomicAdd(&s_words[at - place0], 1u);
+                            }
+                        }
+                    }
+                };
+                for (std::uint32_t q0 = tid; q0 < quads; q0 += kThreads * kQuads) {
+                    uint4 now[kQuads];
 #pragma unroll
-                for (std::uint32_t k = 0; k < 2u; ++k) {
-                    std::uint32_t const marked = bits_of(s_touched, at + k * 128u) & 15u;
-                    if (marked != 0) {
-                        uint4 const w = *reinterpret_cast<uint4 const*>(&s_words[at + k * 128u]);
-                        x[k].x = (marked & 1u) != 0 ? __uint_as_float(w.x) : x[k].x;
-                        x[k].y = (marked & 2u) != 0 ? __uint_as_float(w.y) : x[k].y;
-                        x[k].z = (marked & 4u) != 0 ? __uint_as_float(w.z) : x[k].z;
-                        x[k].w = (marked & 8u) != 0 ? __uint_as_float(w.w) : x[k].w;
+                    for (std::uint32_t k = 0; k < kQuads; ++k) {
+                        now[k] = ahead[k];
+                    }
+                    load_quads(q0 + kThreads * kQuads);
+#pragma unroll
+                    for (std::uint32_t k = 0; k < kQuads; ++k) {
+                        std::uint32_t const i = from + (q0 + k * kThreads) * 4u;
+                        count(now[k].x, i);
+                        count(now[k].y, i + 1u);
+                        count(now[k].z, i + 2u);
+                        count(now[k].w, i + 3u);
                     }
                 }
-            }
-            if (masked) {
-#pragma unroll
-                for (std::uint32_t k = 0; k < 2u; ++k) {
-                    std::uint32_t const allow = blocked ? 0u : bits_of(s_mask, at + k * 128u);
-                    x[k].x = (allow & 1u) != 0 ? x[k].x : -INFINITY;
-                    x[k].y = (allow & 2u) != 0 ? x[k].y : -INFINITY;
-                    x[k].z = (allow & 4u) != 0 ? x[k].z : -INFINITY;
-                    x[k].w = (allow & 8u) != 0 ? x[k].w : -INFINITY;
+                std::uint32_t const edge = tid < from ? tid : from + quads * 4u + (tid - from);
+                if (edge < len && tid < from + 3u) {
+                    count(text[edge], edge);
                 }
-            }
-#pragma unroll
-            for (std::uint32_t k = 0; k < 2u; ++k) {
-                float const high = fmaxf(fmaxf(fmaxf(x[k].x, x[k].y), x[k].z), x[k].w);  // passes NaN over
-                if (high > top) {
-                    top = high;
-                    top_id = v + k * 128u + (x[k].x == high ? 0u : x[k].y == high ? 1u : x[k].z == high ? 2u : 3u);
-                }
-            }
-            if (vector_out) {
-                *reinterpret_cast<float4*>(out + v) = x[0];
-                *reinterpret_cast<float4*>(out + v + 128u) = x[1];
-            } else if (out != nullptr) {
-#pragma unroll
-                for (std::uint32_t k = 0; k < 2u; ++k) {
-                    out[v + k * 128u] = x[k].x;
-                    out[v + k * 128u + 1u] = x[k].y;
-                    out[v + k * 128u + 2u] = x[k].z;
-                    out[v + k * 128u + 3u] = x[k].w;
-                }
+            };
+            if (wide) {
+                scan(std::false_type{});
+            } else {
+                scan(std::true_type{});
             }
         }
-    }
-    if (whole_blocks < blocks) {  // the vocabulary's last, partial block
-        std::uint32_t const at0 = whole_blocks * kBlock;
-        for (std::uint32_t e = tid; token_of(at0) + e < vocab; e += kThreads) {
-            one(at0 + e, token_of(at0) + e);
+        __syncthreads();
+        // A place's word: its count, then its place in the list.
+        auto* const s_half = reinterpret_cast<std::uint16_t*>(s_words);
+        auto word_of = [&](std::uint32_t at) -> std::uint32_t { return wide ? s_words[at - place0] : s_half[at]; };
+        auto set_word = [&](std::uint32_t at, std::uint32_t w) {
+            if (wide) {
+                s_words[at - place0] = w;
+            } else {
+                s_half[at] = static_cast<std::uint16_t>(w);
+            }
+        };
+        std::uint32_t const stop = place0 / kBlock + span / kBlock < blocks ? place0 / kBlock + span / kBlock : blocks;
+        std::uint32_t run = stop;  // blocks at a time
+        for (std::uint32_t block0 = place0 / kBlock; block0 < stop;) {
+            std::uint32_t const block1 = stop - block0 < run ? stop : block0 + run;
+            // ---- the marked tokens' logits
+            if (penal) {
+                // They lie in clumps: a list spreads them over the threads.
+                std::uint32_t const word1 = block1 * (kBlock / 32u);
+                for (std::uint32_t i0 = block0 * (kBlock / 32u); i0 < word1; i0 += kThreads) {
+                    std::uint32_t const w = i0 + tid;
+                    std::uint32_t bits = w < word1 ? s_touched[w] : 0u;
+                    std::uint32_t const own = __popc(bits);
+                    std::uint32_t upto = own;
+#pragma unroll
+                    for (std::uint32_t o = 1; o < 32u; o *= 2u) {
+                        std::uint32_t const x = __shfl_up_sync(0xffffffffu, upto, o);
+                        upto += lane >= o ? x : 0u;
+                    }
+                    std::uint32_t base = 0;
+                    if (lane == 31u && upto != 0) {
+                        base = atomicAdd(&s_listed, upto);
+                    }
+                    std::uint32_t n = __shfl_sync(0xffffffffu, base, 31) + upto - own;
+                    auto list = [&](std::uint32_t at, std::uint32_t place) {
+                        if (place < kListed) {
+                            s_list[place] = static_cast<std::uint16_t>(at);
+                        }
+                    };
+                    // A word with many marks is taken by the whole warp, a lane a bit.
+                    for (std::uint32_t full = __ballot_sync(0xffffffffu, own > 4u); full != 0; full &= full - 1u) {
+                        std::uint32_t const from_lane = __ffs(full) - 1u;
+                        std::uint32_t const word = __shfl_sync(0xffffffffu, bits, from_lane);
+                        std::uint32_t const first = __shfl_sync(0xffffffffu, n, from_lane);
+                        std::uint32_t const at = __shfl_sync(0xffffffffu, w, from_lane) * 32u + lane;
+                        if ((word >> lane & 1u) != 0) {
+                            list(at, first + __popc(word & ((1u << lane) - 1u)));
+                        }
+                    }
+                    // Straight-line: loops of divergent length cost three times as much.
+#pragma unroll
+                    for (std::uint32_t e = 0; e < 4u; ++e) {
+                        if (own <= 4u && bits != 0) {
+                            list(w * 32u + __ffs(bits) - 1u, n++);
+                            bits &= bits - 1u;
+                        }
+                    }
+                }
+                __syncthreads();
+            }
+            std::uint32_t const listed = penal ? s_listed : 0u;
+            if (listed + (b1 - b0) > kListed && run > kFewBlocks) {
+                run = kFewBlocks;
+                __syncthreads();
+                if (tid == 0) {
+                    s_listed = 0;
+                }
+                __syncthreads();
+                continue;
+            }
+            if (penal) {
+                for (std::uint32_t i0 = tid; i0 < listed; i0 += kThreads * kGather) {
+                    std::uint32_t at[kGather];
+                    float x[kGather];
+#pragma unroll
+                    for (std::uint32_t k = 0; k < kGather; ++k) {
+                        std::uint32_t const i = i0 + k * kThreads;
+                        at[k] = i < listed ? s_list[i] : 0u;
+                        x[k] = i < listed ? in[first_of(at[k] / kBlock) + at[k] % kBlock] : 0.f;
+                    }
+#pragma unroll
+                    for (std::uint32_t k = 0; k < kGather; ++k) {
+                        std::uint32_t const i = i0 + k * kThreads;
+                        if (i < listed) {
+                            std::uint32_t const n = word_of(at[k]);
+                            float y = x[k] > 0.f ? __fdiv_rn(x[k], rep) : __fmul_rn(x[k], rep);
+                            if (n != 0) {
+                                y = __fsub_rn(y, __fmul_rn(freq, static_cast<float>(n)));
+                                y = __fsub_rn(y, pres);
+                            }
+                            s_value[i] = y;
+                            set_word(at[k], i);
+                        }
+                    }
+                }
+                __syncthreads();
+            }
+            if (biased) {
+                for (std::uint32_t i = b0 + tid; i < b1; i += kThreads) {
+                    if (i != b0 + tid || block0 != 0) {
+                        load_bias(i);
+                    }
+                    std::uint32_t const v = bias_token;
+                    if (bias_next < v) {
+                        report(kErrBadArgument);
+                    }
+                    if (owned(v) && bias_next != v) {
+                        std::uint32_t const at = place_of(v);
+                        if (at / kBlock - block0 < block1 - block0) {
+                            if ((s_touched[at / 32u] >> (at % 32u) & 1u) != 0) {
+                                float& y = s_value[word_of(at)];
+                                y = __fadd_rn(y, bias_value);
+                            } else {
+                                std::uint32_t const place = atomicAdd(&s_listed, 1u);
+                                if (place < kListed) {  // as ever, unless ids descend
+                                    s_value[place] = __fadd_rn(bias_logit, bias_value);
+                                    set_word(at, place);
+                                    atomicOr(&s_touched[at / 32u], 1u << (at % 32u));
+                                }
+                            }
+                        }
+                    }
+                }
+                __syncthreads();
+            }
+            // ---- the logits
+            // A warp takes a block of 256 tokens: two steps of four for every thread.
+            auto stream = [&](std::uint32_t block, auto inner) {
+                std::uint32_t const u0 = first_of(block) + lane * 4u;
+                std::uint32_t const at = block * kBlock + lane * 4u;
+                bool const whole[2] = {inner || (u0 >= shift && u0 + 4u <= end), inner || u0 + 132u <= end};
+                float x[8];
+#pragma unroll
+                for (std::uint32_t k = 0; k < 2u; ++k) {
+                    float const* const src = in + u0 + k * 128u;
+                    if (whole[k]) {
+                        float4 const v = *reinterpret_cast<float4 const*>(src);
+                        x[4u * k] = v.x;
+                        x[4u * k + 1u] = v.y;
+                        x[4u * k + 2u] = v.z;
+                        x[4u * k + 3u] = v.w;
+                    } else {
+#pragma unroll
+                        for (std::uint32_t e = 0; e < 4u; ++e) {
+                            std::uint32_t const u = u0 + k * 128u + e;
+                            x[4u * k + e] = u >= shift && u < end ? src[e] : -INFINITY;
+                        }
+                    }
+                }
+                if (penal || biased) {
+#pragma unroll
+                    for (std::uint32_t k = 0; k < 2u; ++k) {
+                        std::uint32_t const marked = bits_of(s_touched, at + k * 128u) & 15u;
+                        if (marked != 0) {
+                            std::uint32_t w[4];
+                            if (wide) {
+                                uint4 const v = *reinterpret_cast<uint4 const*>(&s_words[at + k * 128u - place0]);
+                                w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+                            } else {
+                                uint2 const v = *reinterpret_cast<uint2 const*>(&s_half[at + k * 128u]);
+                                w[0] = v.x & 0xffffu, w[1] = v.x >> 16, w[2] = v.y & 0xffffu, w[3] = v.y >> 16;
+                            }
+#pragma unroll
+                            for (std::uint32_t e = 0; e < 4u; ++e) {
+                                if ((marked >> e & 1u) != 0) {
+                                    x[4u * k + e] = s_value[w[e]];
+                                }
+                            }
+                        }
+                    }
+                }
+                if (masked) {
+#pragma unroll
+                    for (std::uint32_t k = 0; k < 2u; ++k) {
+                        std::uint32_t const allow = blocked ? 0u : bits_of(s_mask, at + k * 128u);
+#pragma unroll
+                        for (std::uint32_t e = 0; e < 4u; ++e) {
+                            x[4u * k + e] = (allow >> e & 1u) != 0 ? x[4u * k + e] : -INFINITY;
+                        }
+                    }
+                }
+                float high[2];  // of each step; fmaxf passes NaN over
+#pragma unroll
+                for (std::uint32_t k = 0; k < 2u; ++k) {
+                    high[k] = fmaxf(fmaxf(x[4u * k], x[4u * k + 1u]), fmaxf(x[4u * k + 2u], x[4u * k + 3u]));
+                }
+                if (fmaxf(high[0], high[1]) > top) {
+                    top = fmaxf(high[0], high[1]);
+                    std::uint32_t e = 7;
+#pragma unroll
+                    for (std::uint32_t i = 7; i-- > 0;) {
+                        e = x[i] == top ? i : e;
+                    }
+                    top_id = u0 + e % 4u + e / 4u * 128u;
+                }
+                if (out != nullptr) {
+#pragma unroll
+                    for (std::uint32_t k = 0; k < 2u; ++k) {
+                        float const* const y = x + 4u * k;
+                        std::uint32_t const u = u0 + k * 128u;
+                        if (vector_out && whole[k]) {
+                            *reinterpret_cast<float4*>(out + u) = make_float4(y[0], y[1], y[2], y[3]);
+                        } else {
+#pragma unroll
+                            for (std::uint32_t e = 0; e < 4u; ++e) {
+                                if (u + e >= shift && u + e < end) {
+                                    out[u + e] = y[e];
+                                }
+                            }
+                        }
+                    }
+                }
+            };
+            for (std::uint32_t block = block0 + warp; block < block1; block += kWarps) {
+                std::uint32_t const u = first_of(block);
+                if (u >= shift && u + kBlock <= end) {
+                    stream(block, std::true_type{});
+                } else {  // the row's first and last
+                    stream(block, std::false_type{});
+                }
+            }
+            block0 = block1;
+            if (block0 < stop) {
+                __syncthreads();
+                if (tid == 0) {
+                    s_listed = 0;
+                }
+                __syncthreads();
+            }
         }
     }
 
@@ -478,8 +564,7 @@ __global__ void __launch_bounds__(kThreads, 4) logits_process_kernel(const __gri
     if (d.tokens == nullptr) {
         return;
     }
-    std::uint64_t const whole = candidate(top, top_id);
-    best = whole > best ? whole : best;
+    std::uint64_t best = candidate(top, top_id - shift);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         std::uint64_t const other = __shfl_xor_sync(0xffffffffu, best, o);
@@ -496,16 +581,16 @@ __global__ void __launch_bounds__(kThreads, 4) logits_process_kernel(const __gri
     }
     if (lc != 0) {
         cluster_wait();
-        if (tid == 0 && rank != 0) {
-            st_cluster_u64(cluster_map(&s_cluster[rank], 0), best);
+        if (tid == 0) {
+            if (rank != 0) {
+                st_cluster_u64(cluster_map(&s_cluster[rank], 0), best, cluster_map(&s_winners, 0));
+            } else {
+                mbar_wait(&s_winners, 0, &g_logits_status);
+            }
         }
-        // Only the first CTA waits; the others are done once they said so.
-        __syncwarp();
-        cluster_arrive();
         if (rank != 0) {
             return;
         }
-        cluster_wait();
     }
     if (tid == 0) {
         for (std::uint32_t r = 1; r < 1u << lc; ++r) {
@@ -583,19 +668,25 @@ extern "C" int kk_logits_process(const kk_logits_desc* d, void* stream)
     while ((1u << a.cluster_log2) < kMaxCluster && (d->vocab >> a.cluster_log2) > 4096u) {
         ++a.cluster_log2;
     }
-    std::uint32_t const blocks = (d->vocab + kBlock - 1u) / kBlock;
-    a.capacity = (((blocks - 1u) >> a.cluster_log2) + 1u) * kBlock;
+    // A row that does not start on a 16-byte boundary reaches up to 3 places further.
+    std::uint32_t const blocks = (d->vocab + 3u + kBlock - 1u) / kBlock;
+    a.capacity = ((((blocks - 1u) >> a.cluster_log2) + 2u) & ~1u) * kBlock;
     std::uint64_t bytes = 0;
+    auto reserve = [&](std::uint64_t n) {
+        std::uint64_t const at = bytes / 4u;
+        bytes += n;
+        return static_cast<std::uint32_t>(at);
+    };
     if (words) {
-        a.touched_at = a.capacity + 4u;
-        a.list_at = a.touched_at + a.capacity / 32u + 1u;
-        bytes = (std::uint64_t(a.list_at) + kListed / 2u) * 4u;
+        reserve(a.capacity * 2u);
+        a.touched_at = reserve(a.capacity / 8u);
+        a.value_at = reserve(kListed * 4u);
+        a.list_at = reserve(kListed * 2u);
     }
     if (d->mask != nullptr) {
-        a.mask_at = static_cast<std::uint32_t>(bytes / 4u);
-        bytes += a.capacity / 8u;
+        a.mask_at = reserve(a.capacity / 8u);
     }
-    if (bytes > kMaxSharedBytes || (words && a.capacity + 4u > 65536u)
+    if (bytes > kMaxSharedBytes || (words && d->vocab > kMaxWordsVocab) || (d->mask != nullptr && d->vocab > kMaxVocab)
         || (std::uint64_t(d->rows) << a.cluster_log2) > 0x7fffffffu) {
         return KK_EINVAL;
     }

@@ -236,6 +236,21 @@ def test_logits_specials_masks_and_ties(kk):
 
 
 @gpu_test
+@pytest.mark.parametrize("rows,vocab,lens", [
+    (2, 33000, (70001, 65536)),      # counts beyond 16 bits
+    (3, 50021, (30000, 65535, 90000)),  # more distinct tokens than a list of them holds
+    (2, 300, (66000, 1)), (1, 4097, (131072,)), (2, 131072, (131072, 20)),
+], ids=str)
+@pytest.mark.parametrize("in_place", [False, True])
+def test_logits_long_histories(kk, rows, vocab, lens, in_place):
+    c = Case(rows, vocab, seed=vocab, stride=vocab + 1)
+    c.with_history(lens, prompts=[min(n // 50, 100) for n in lens]).with_mask(0.8)
+    c.history[0][:66000] = vocab // 3  # one token, more often than 16 bits count
+    c.with_bias([vocab // 2, 0, 40][:rows])
+    c.check(kk, in_place=in_place)
+
+
+@gpu_test
 def test_logits_repeated_ids_and_ids_outside_the_vocabulary(kk):
     c = Case(3, 5000, seed=6)
     c.with_history([4000, 4000, 4000], prompts=[0, 4000, 2000])
