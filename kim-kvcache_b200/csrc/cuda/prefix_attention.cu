@@ -32,11 +32,17 @@
 // grows by more than 2^8 (P stays within FP16; the quotient is exact in either
 // case).
 // The exponentials, 16 per SM and clock, bound a K/V tile for 256 rows: 2,048
-// clocks. Measured steps, per such tile: 2.6 us with two groups that waited for
-// each product (or four of half rows), while the products were issued from a branch
-// of one lane (see elect_lane); 1.9 us without that branch; 1.6 us without the
-// low halves; 1.4 us with the third S tile. (Four groups in turn over three S
-// tiles: 2.4 us, all three are then in use at once.)
+// clocks, or 1,536 with a quarter of them on the FMA pipes. Measured: 2,500 clocks
+// (64 lanes over each of two prefixes of 32,749 tokens: 57 us); in the loop the
+// exponential unit is busy for 63 % of the time, issue slots for 59 %, the tensor
+// cores for 42 %; of a group's turn of 2,500 clocks 200 go by until it has seen its
+// scores, 150 until it holds them, 400 for the maximum, 1,450 for the weights, 300
+// until it looks for the next. Steps on the way, per such tile: 2.6 us with two groups that
+// waited for each product (or four of half rows), while the products were issued
+// from a branch of one lane (see elect_lane); 1.9 us without that branch; 1.6 us
+// without the low halves; 1.4 us with the third S tile. No faster: four groups in
+// turn over three S tiles (2.4 us, all three are then in use at once), 16 softmax
+// warps with a quarter of two rows a thread (1.7 us), an issuer for each group.
 //
 // A lane's own pages: one warp per (lane, KV head, run of pages), 16-token
 // slices through a private cp.async ring, scores transposed (tokens x heads) on
