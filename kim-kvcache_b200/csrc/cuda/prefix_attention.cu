@@ -1654,13 +1654,17 @@ int kk_prefix_attention(const kk_prefix_attn_desc* d, void* stream)
             // A pool without pages keeps an empty map: no descriptor selects it.
             if ((a.micro_slots != 0
                     && (!encodePageHeadMap(&maps.micro8, a.micro, a.micro_slots, a.micro_cap, d->pools.layers, heads, 8)
-                        || !encodePageHeadMap(&maps.micro, a.micro, a.micro_slots, a.micro_cap, d->pools.layers, heads,
-                            a.micro_cap)))
+                        || (a.micro_cap != 8u
+                            && !encodePageHeadMap(&maps.micro, a.micro, a.micro_slots, a.micro_cap, d->pools.layers,
+                                heads, a.micro_cap))))
                 || (a.extent_slots != 0
                     && (!encodePageHeadMap(&maps.extent8, a.extent, a.extent_slots, 64, d->pools.layers, heads, 8)
                         || !encodePageHeadMap(&maps.extent, a.extent, a.extent_slots, 64, d->pools.layers, heads,
                             64)))) {
                 return KK_EINVAL;
+            }
+            if (a.micro_cap == 8u) {
+                maps.micro = maps.micro8;
             }
         }
         std::uint32_t const own = d->plan.num_items - d->plan.num_shared;
