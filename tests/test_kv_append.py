@@ -277,3 +277,42 @@ def test_append_reports_bad_rows_and_leaves_them(kk):
             assert bool((micro == 0).all()) and bool((out == 3.0).all())
         else:  # cos 1, sin 0: copied
             assert torch.equal(out[0], x[0, :D]) and int((micro != 0).sum()) == int((x[0, D:] != 0).sum())
+
+
+@gpu_test
+def test_append_behind_32_bit_offsets(kk):
+    """Rows of queries, and a page, that begin more than 2^32 elements behind their arrays' start."""
+    layers, page, hkv, hq, rows = 2, 64, 16, 2, 3
+    slot, stride = 16400, (1 << 31) + 8
+    pool = torch.empty(slot + 1, layers, 2, page, hkv, 64, dtype=torch.half, device="cuda")
+    pool[slot:] = 7.0
+    q = torch.empty(2 * stride + hq * 64, dtype=torch.half, device="cuda")
+    rng = np.random.RandomState(20)
+    x = rng.randn(rows, hq + 2 * hkv, 64).astype(np.float16)
+    for r in range(rows):
+        q[r * stride:r * stride + hq * 64] = torch.from_numpy(x[r, :hq].reshape(-1)).cuda()
+    kv = torch.from_numpy(x[:, hq:].reshape(rows, -1)).cuda()
+    slots = to_device_bytes((kk.KvSlot * rows)(*[kk.KvSlot(slot, t, 0, 1) for t in (63, 0, 5)]))
+    positions = np.array([9, 1000, 3], np.uint32)
+    d_pos = torch.from_numpy(positions.view(np.int32)).cuda()
+    d = kk.KvAppendDesc()
+    d.pools = kk.KvPools(p(pool), 0, slot + 1, 0, layers, hkv, 64, page)
+    d.layer, d.rows, d.q_heads, d.rotary_dim, d.theta = 1, rows, hq, 64, 10000.0
+    d.slots, d.positions = p(slots), p(d_pos)
+    d.query = d.query_out = p(q)
+    d.query_stride = d.query_out_stride = stride
+    d.key, d.value = p(kv), p(kv) + 2 * 64 * hkv
+    d.key_stride = d.value_stride = kv.shape[1]
+    torch.cuda.synchronize()
+    assert kk.kernels()["kv_append_rope"](C.byref(d), None) == 0
+    torch.cuda.synchronize()
+    assert kk.kernels()["device_status"](None) == 0
+    got_q = np.stack([q[r * stride:r * stride + hq * 64].cpu().numpy() for r in range(rows)]).reshape(rows, hq, 64)
+    page_now = pool[slot].cpu().numpy()
+    got_k = page_now[1, 0, [63, 0, 5]]
+    got = np.concatenate([got_q, got_k], 1)
+    turned = x[:, :hq + hkv]
+    ab = np.abs(turned[..., :32].astype(float)) + np.abs(turned[..., 32:].astype(float))
+    assert_rounded(got, rotate_ref(turned, positions, 64, 10000.0), np.concatenate([ab, ab], -1))
+    assert np.array_equal(page_now[1, 1, [63, 0, 5]], x[:, hq + hkv:])
+    assert (page_now[0] == 7).all() and (np.delete(page_now[1], [63, 0, 5], 1) == 7).all()

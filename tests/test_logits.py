@@ -318,3 +318,31 @@ def test_logits_on_streams_captured_and_repeated(kk):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, x) and torch.equal(tokens.long(), x.argmax(-1))
+
+
+@gpu_test
+def test_logits_behind_32_bit_offsets(kk):
+    """Rows that begin more than 2^32 elements behind the array's start (17 GB), in place."""
+    rows, vocab, stride = 3, 5000, (1 << 31) + 1
+    x = torch.empty(2 * stride + vocab, device="cuda")
+    rng = np.random.RandomState(21)
+    host = rng.randn(rows, vocab).astype(np.float32)
+    for r in range(rows):
+        x[r * stride:r * stride + vocab] = torch.from_numpy(host[r]).cuda()
+    banned = torch.tensor([int(t) for t in host.argmax(1)], dtype=torch.int32, device="cuda")
+    offsets = torch.arange(rows + 1, dtype=torch.int32, device="cuda")
+    values = torch.full((rows,), -100.0, device="cuda")
+    tokens = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    d = kk.LogitsDesc()
+    d.logits = d.out = p(x)
+    d.logits_stride = d.out_stride = stride
+    d.rows, d.vocab, d.tokens = rows, vocab, p(tokens)
+    d.bias_tokens, d.bias_values, d.bias_offsets, d.bias_size = p(banned), p(values), p(offsets), rows
+    torch.cuda.synchronize()
+    assert kk.kernels()["logits_process"](C.byref(d), None) == 0
+    torch.cuda.synchronize()
+    assert kk.kernels()["device_status"](None) == 0
+    for r in range(rows):
+        host[r, host[r].argmax()] += np.float32(-100.0)
+        assert np.array_equal(x[r * stride:r * stride + vocab].cpu().numpy(), host[r])
+    assert np.array_equal(tokens.cpu().numpy(), host.argmax(1))

@@ -450,6 +450,18 @@ def test_prefix_chunk_positions_share_pages(kk):
 
 
 @gpu_test
+@pytest.mark.parametrize("page", [8, 64])
+def test_prefix_pages_behind_32_bit_offsets(kk, page):
+    """Pages that begin more than 2^32 elements behind the pool's start (an 8.6 GB pool)."""
+    pages = Pages(random.Random(19), page)
+    pages.next = [0, 16400] if page == 8 else [16400, 0]
+    s = Setup(kk, forks(pages, 300, [20, 0, 70]), pages, 32, 16, 20)
+    assert (s.extent if page == 8 else s.micro)[16400:].data_ptr() - p(s.extent if page == 8 else s.micro) > 2 ** 33
+    s.run()
+    s.check()
+
+
+@gpu_test
 def test_prefix_matches_per_lane_attention(kk):
     K = kk.kernels()
     pages = Pages(random.Random(12))

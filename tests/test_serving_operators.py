@@ -209,7 +209,9 @@ def test_decode_steps_of_forked_lanes(kk, hq, hkv, page, extents):
                 assert s.K[name](C.byref(desc), on) == 0, name
 
         torch.cuda.synchronize()
+        s.K["set_pdl"](step % 2)
         run(stream.cuda_stream)
+        s.K["set_pdl"](0)
         torch.cuda.synchronize()
         assert s.K["device_status"](None) == 0
         s.check_append(last, positions, places, [True] * rows)
@@ -218,9 +220,12 @@ def test_decode_steps_of_forked_lanes(kk, hq, hkv, page, extents):
         chosen = s.check_choose()
         if step % 4 == 0:  # the step as one graph, twice: the same bits
             kept = [t.clone() for t in (s.q, s.out, s.logits, s.processed, s.tokens)]
+            # Launched ahead of each other's ends as well (programmatic dependents).
+            s.K["set_pdl"](int(step > 0))
             graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(graph, stream=stream):
                 run(stream.cuda_stream)
+            s.K["set_pdl"](0)
             for _ in range(2):
                 for t in (s.q, s.out, s.logits, s.processed, s.tokens):
                     t.fill_(3)
