@@ -131,6 +131,8 @@ __global__ void kv_copy_kernel(PoolView v, std::uint32_t layer_begin, kk_kv_copy
 
 constexpr std::uint32_t kMaxRotaryDim = 256;
 constexpr int kAppendThreads = 256;
+constexpr std::uint32_t kAppendWave = 148 * 5;  // CTAs that the SMs hold at once
+constexpr std::uint32_t kTailBatch = 3;  // copies in flight per thread (one: 16.0 us, three: 14.6, for 4,999 half rotated rows)
 constexpr std::uint32_t kAppendMaxRows = 8;  // rows per CTA, at most
 
 struct AppendArgs {
@@ -167,8 +169,8 @@ struct AppendArgs {
 // run under that arithmetic. Angles: position * turns in 64-bit fixed point
 // drops whole turns exactly, and the top 32 bits of what is left are the
 // angle to 2^-32 turns at any position. Five CTAs per SM: the registers that
-// the compiler takes without that bound leave four, 74.8 us in place of 73.6
-// and 19.8 in place of 16.3 at the sizes of a ragged prefill.
+// the compiler takes without that bound leave four (74.8 us in place of 73.6 for
+// 16,384 rows, 19.8 in place of 16.3 for 4,999).
 __global__ void __launch_bounds__(kAppendThreads, 5) kv_append_rope_kernel(const __grid_constant__ AppendArgs a)
 {
     // (cos, sin) of a row's pairs, two to a 16-byte entry: [row][entry of a step][step], so
@@ -310,18 +312,33 @@ __global__ void __launch_bounds__(kAppendThreads, 5) kv_append_rope_kernel(const
     std::uint32_t const tail = a.head_dim - 2u * half;
     std::uint32_t const head_copies = tail / 8u;
     std::uint32_t const row_tails = (a.q_heads + a.kv_heads) * head_copies;
-    for (std::uint32_t i = tid; i < n_rows * row_tails; i += kAppendThreads) {
-        std::uint32_t const row = i / row_tails;
-        std::uint32_t const rest = i - row * row_tails;
-        std::uint32_t const head = rest / head_copies;
-        std::uint32_t const e = 2u * half + (rest - head * head_copies) * 8u;
-        __half* dst = s_dst[row];
-        if (dst == nullptr) {
-            continue;
+    std::uint32_t const tails = n_rows * row_tails;
+    for (std::uint32_t i0 = tid; i0 < tails; i0 += kAppendThreads * kTailBatch) {
+        uint4 x[kTailBatch];
+        __half* to[kTailBatch];
+#pragma unroll
+        for (std::uint32_t k = 0; k < kTailBatch; ++k) {
+            std::uint32_t const i = i0 + k * kAppendThreads;
+            to[k] = nullptr;
+            if (i < tails) {
+                std::uint32_t const row = i / row_tails;
+                std::uint32_t const rest = i - row * row_tails;
+                std::uint32_t const head = rest / head_copies;
+                std::uint32_t const e = 2u * half + (rest - head * head_copies) * 8u;
+                __half* const dst = s_dst[row];
+                if (dst != nullptr) {
+                    to[k] = head < a.q_heads ? a.query_out + (row0 + row) * a.query_out_stride + head * a.head_dim + e
+                                             : dst + (head - a.q_heads) * a.head_dim + e;
+                    x[k] = *reinterpret_cast<uint4 const*>(source(Step{row, head, e}));
+                }
+            }
         }
-        dst = head < a.q_heads ? a.query_out + (row0 + row) * a.query_out_stride + head * a.head_dim + e
-                               : dst + (head - a.q_heads) * a.head_dim + e;
-        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4 const*>(source(Step{row, head, e}));
+#pragma unroll
+        for (std::uint32_t k = 0; k < kTailBatch; ++k) {
+            if (to[k] != nullptr) {
+                *reinterpret_cast<uint4*>(to[k]) = x[k];
+            }
+        }
     }
 }
 
@@ -494,11 +511,12 @@ int kk_kv_append_rope(const kk_kv_append_desc* d, void* stream)
     a.pools = view(d->pools);
     a.layer = d->layer;
     a.rows = d->rows;
-    // Few rows: one CTA each, for the shortest chain of loads (a decode batch
-    // of 64 rows: 2.9 us, 3.7 with four rows per CTA). Many: enough rows per CTA
-    // that its threads take several steps each (16,384 rows of 32 + 8 heads of
-    // 128: 73.6 us, 74.7 with two rows).
-    a.rows_per_cta = d->rows <= 1024u ? 1u : 4u;
+    // One wave of CTAs where their tables hold the rows, each row's chain of loads
+    // as short as that allows (a decode batch of 64 rows: 2.9 us, 3.7 with four rows
+    // per CTA; 4,999 rows of 16 + 2 heads of 128, half rotated: 12.8 us, 14.6 with
+    // four). More rows: many waves, of four rows per CTA (16,384 rows of 32 + 8
+    // heads of 128: 72.5 us, 74.4 with five, 76.8 with seven).
+    a.rows_per_cta = d->rows <= kAppendWave * kAppendMaxRows ? (d->rows - 1u) / kAppendWave + 1u : 4u;
     a.q_heads = d->q_heads;
     a.kv_heads = d->pools.kv_heads;
     a.head_dim = d->pools.head_dim;

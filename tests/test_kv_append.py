@@ -100,6 +100,12 @@ CASES = [
     (2, 2, 2, 320, 256, 8, True, 70),
     (1025, 6, 2, 64, 48, 8, True, 8192),
     (1500, 32, 8, 128, 128, 8, True, 1 << 20),
+    # Rows per thread block: one wave of blocks holds 740, 5,920 at most.
+    (740, 2, 1, 16, 16, 8, True, 100),
+    (741, 2, 1, 32, 16, 8, True, 100),
+    (4999, 4, 2, 128, 64, 16, False, 100000),
+    (5920, 2, 1, 16, 16, 8, True, 100),
+    (5921, 3, 1, 24, 16, 8, True, 100),
 ]
 
 
