@@ -1147,7 +1147,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_attention_kernel(const __g
 // ---- joining the partials -----------------------------------------------------
 
 constexpr std::uint32_t kJoinThreads = 256;
-constexpr std::uint32_t kJoinBatch = 8;  // partials requested at once
+constexpr std::uint32_t kJoinBatch = 10;  // partials that each half of the warp requests at once
 
 // A warp per query row: out = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i over the
 // row's partials. 16 lanes hold 4 dims each; the two halves of the warp take
@@ -1202,12 +1202,13 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(const __grid_
         acc.z = acc.z * f + o.z * f1;
         acc.w = acc.w * f + o.w * f1;
     };
-    for (std::uint32_t i0 = t % 32u / 16u; i0 < count; i0 += 2u * kJoinBatch) {
+    for (std::uint32_t first = 0; first < count; first += 2u * kJoinBatch) {
         float2 ml[kJoinBatch];
         float4 o[kJoinBatch];
+        float top = m;
 #pragma unroll
         for (std::uint32_t k = 0; k < kJoinBatch; ++k) {
-            std::uint32_t const i = i0 + 2u * k;
+            std::uint32_t const i = first + 2u * k + t % 32u / 16u;
             ml[k] = make_float2(-INFINITY, 0.f);
             o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
             if (i < count) {
@@ -1218,7 +1219,23 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(const __grid_
         }
 #pragma unroll
         for (std::uint32_t k = 0; k < kJoinBatch; ++k) {
-            add(ml[k].x, ml[k].y, o[k]);
+            top = fmaxf(top, ml[k].x);
+        }
+        float const use = top == -INFINITY ? 0.f : top;
+        float const f = exp2_approx(m - use);
+        m = top;
+        l *= f;
+        acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+#pragma unroll
+        for (std::uint32_t k = 0; k < kJoinBatch; ++k) {
+            if (first + 2u * k < count) {  // the same for the whole warp
+                float const f1 = exp2_approx(ml[k].x - use);
+                l += ml[k].y * f1;
+                acc.x += o[k].x * f1;
+                acc.y += o[k].y * f1;
+                acc.z += o[k].z * f1;
+                acc.w += o[k].w * f1;
+            }
         }
     }
     // The upper half's part joins the lower's.
@@ -1271,14 +1288,16 @@ cudaError_t allowSharedMemory()
 // ---- planning -------------------------------------------------------------------
 
 // Measured times of a thread block, in nanoseconds, from which the plan deals
-// the SMs out between the prefixes and the lanes' own pages.
+// the SMs out between the prefixes and the lanes' own pages. (Those of own items
+// with the cost of joining their parts: shorter items than these give are no
+// faster, 13.9 us in place of 13.0 for 32 lanes with up to 1,024 tokens.)
 constexpr double kSharedNs = 5500.;     // a shared item without its tiles
 constexpr double kTilePairNs = 1450.;   // a 128-token tile for two row tiles
 constexpr double kTileSingleNs = 750.;  // for one
 constexpr double kOwnNs = 1000.;        // a block of lanes' own items without them
-constexpr double kTaskNs = 2200.;       // an own item without its tokens
-constexpr double kTaskTokenNs = 28.;     // a token of an own item, by its warp
-constexpr double kOwnTokenNs = 6.;      // the same by the block: 256 bytes at an SM's share of HBM
+constexpr double kTaskNs = 3000.;       // an own item without its tokens
+constexpr double kTaskTokenNs = 40.;     // a token of an own item, by its warp
+constexpr double kOwnTokenNs = 4.;      // the same by the block: 256 bytes at an SM's share of HBM
 constexpr std::uint32_t kOwnMinTokens = 64;
 
 std::uint32_t groupsOf(kk_page_desc const& d) { return d.valid_tokens > 64u ? 0u : (d.valid_tokens + 7u) / 8u; }
