@@ -171,6 +171,11 @@ struct AppendArgs {
 // angle to 2^-32 turns at any position. Five CTAs per SM: the registers that
 // the compiler takes without that bound leave four (74.8 us in place of 73.6 for
 // 16,384 rows, 19.8 in place of 16.3 for 4,999).
+// kWhole: every dim of a head is rotated. Inputs then go around L1 (16,384 rows:
+// 69.5 us in place of 72.5); beside copied dims that costs more than it gives (4,999
+// half rotated rows: 13.9 us in place of 12.7). The loop over copied dims, which
+// then has no turns, stays: without it the compiler spills (75.4 us).
+template <bool kWhole>
 __global__ void __launch_bounds__(kAppendThreads, 5) kv_append_rope_kernel(const __grid_constant__ AppendArgs a)
 {
     // (cos, sin) of a row's pairs, two to a 16-byte entry: [row][entry of a step][step], so
@@ -213,16 +218,20 @@ __global__ void __launch_bounds__(kAppendThreads, 5) kv_append_rope_kernel(const
         return a.value + (row0 + row) * a.value_stride + (i - row * row_copies) * 8u;
     };
 
+    auto load = [](__half const* src) {
+        uint4 const* const p = reinterpret_cast<uint4 const*>(src);
+        return kWhole ? __ldcg(p) : *p;
+    };
     Step cur{};
     uint4 lo{}, hi{}, val{};
     if (tid < steps) {
         cur = locate(tid);
         __half const* src = source(cur);
-        lo = *reinterpret_cast<uint4 const*>(src);
-        hi = *reinterpret_cast<uint4 const*>(src + half);
+        lo = load(src);
+        hi = load(src + half);
     }
     if (tid < copies) {
-        val = *reinterpret_cast<uint4 const*>(value_source(tid));
+        val = load(value_source(tid));
     }
 
     if (tid < n_rows) {
@@ -267,8 +276,8 @@ __global__ void __launch_bounds__(kAppendThreads, 5) kv_append_rope_kernel(const
         if (next < steps) {
             cur = locate(next);
             __half const* src = source(cur);
-            lo = *reinterpret_cast<uint4 const*>(src);
-            hi = *reinterpret_cast<uint4 const*>(src + half);
+            lo = load(src);
+            hi = load(src + half);
         }
         i = next;
         __half* dst = s_dst[s.row];
@@ -301,7 +310,7 @@ __global__ void __launch_bounds__(kAppendThreads, 5) kv_append_rope_kernel(const
         uint4 const x = val;
         i += kAppendThreads;
         if (i < copies) {
-            val = *reinterpret_cast<uint4 const*>(value_source(i));
+            val = load(value_source(i));
         }
         __half* dst = s_dst[row];
         if (dst != nullptr) {
@@ -515,7 +524,7 @@ int kk_kv_append_rope(const kk_kv_append_desc* d, void* stream)
     // as short as that allows (a decode batch of 64 rows: 2.9 us, 3.7 with four rows
     // per CTA; 4,999 rows of 16 + 2 heads of 128, half rotated: 12.8 us, 14.6 with
     // four). More rows: many waves, of four rows per CTA (16,384 rows of 32 + 8
-    // heads of 128: 72.5 us, 74.4 with five, 76.8 with seven).
+    // heads of 128: 72.5 us, 74.4 with five, 76.8 with seven, before loads went around L1).
     a.rows_per_cta = d->rows <= kAppendWave * kAppendMaxRows ? (d->rows - 1u) / kAppendWave + 1u : 4u;
     a.q_heads = d->q_heads;
     a.kv_heads = d->pools.kv_heads;
@@ -532,7 +541,8 @@ int kk_kv_append_rope(const kk_kv_append_desc* d, void* stream)
     a.value_stride = d->value_stride;
     a.query_out_stride = d->query_out_stride;
     unsigned const grid = (d->rows - 1u) / a.rows_per_cta + 1u;
-    return static_cast<int>(launch(kv_append_rope_kernel, dim3(grid), dim3(kAppendThreads), 0,
+    return static_cast<int>(launch(
+        d->rotary_dim == d->pools.head_dim ? kv_append_rope_kernel<true> : kv_append_rope_kernel<false>, dim3(grid), dim3(kAppendThreads), 0,
         static_cast<cudaStream_t>(stream), 1, a));
 }
 
