@@ -100,6 +100,10 @@ static_assert(kSliceRing <= 9, "the validity queue below holds eight slices");
 constexpr std::uint32_t kPoly = 1, kPolyOf = 4;
 
 constexpr float kRescale = 8.f;  // log2 growth of a row maximum that rescales O
+// Shared tokens' weights are 2^7 times as large as the maximum asks for: with that growth
+// they still stay below FP16's 2^16, and only those below 2^-21 of the largest one
+// fall among its subnormals.
+constexpr float kWeightLog2 = 7.f;
 
 struct Args {
     __half const* micro;
@@ -658,7 +662,7 @@ __device__ __forceinline__ void soften(Args const& a, kk_prefix_item const& item
             }
             // A NaN or +inf among the scores makes the row NaN, whichever way its
             // weight is computed.
-            float const shift = !(mt < INFINITY) ? NAN : m == -INFINITY ? 0.f : -m;
+            float const shift = !(mt < INFINITY) ? NAN : m == -INFINITY ? 0.f : kWeightLog2 - m;
             std::uint64_t const scale2 = pack_f32x2(a.scale_log2, a.scale_log2);
             std::uint64_t const shift2 = pack_f32x2(shift, shift);
             std::uint64_t sum2[2] = {0, 0};
@@ -754,7 +758,7 @@ __device__ __forceinline__ void soften(Args const& a, kk_prefix_item const& item
             }
         }
         if (mine) {
-            a.part_ml[first_row + r] = make_float2(m, l);
+            a.part_ml[first_row + r] = make_float2(m - kWeightLog2, l);
         }
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");

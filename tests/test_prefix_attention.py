@@ -396,6 +396,35 @@ def test_prefix_many_groups_and_lanes_without_one(kk):
 
 
 @gpu_test
+@pytest.mark.parametrize("score", [6.0, 9.0, 10.5, 11.0, 12.0, 13.0, 14.0])
+def test_prefix_one_token_outweighs_the_rest(kk, score):
+    """A first token with a score far above all others' (which are 0) and no value of its own: what is left
+    of the result are the others' weights, e^-score each, and rounds no worse than any weight does."""
+    pages = Pages(random.Random(21))
+    tables = forks(pages, 4000, [0, 0])
+    s = Setup(kk, tables, pages, 8, 1, 22, sms=1)  # one part: the others stand next to it
+    for pool in (s.micro, s.extent):
+        for part, value in ((0, 0.0), (1, 1.0)):
+            x = pool[:, :, part]
+            x[~torch.isnan(x)] = value
+    slot, _, _, kind = tables[0][0]
+    first = (s.extent if kind else s.micro)[slot, :, :, 0]
+    first.zero_()
+    first[:, 0, :, 0] = score / s.scale
+    s.q.zero_()
+    s.q.view(2, -1)[:, :512:64] = 1.0
+    s.run()
+    torch.cuda.synchronize()
+    assert kk.kernels()["device_status"](None) == 0
+    rest = 3999 * torch.exp(torch.tensor(-score, dtype=torch.float64))
+    want = float(rest / (1 + rest))
+    error = (s.out[:, :512].double() / want - 1).abs().max()
+    # A weight and the result in FP16, half a step each; exponentials, their argument (off by 2^-24 of 21) and
+    # FP32 sums of 4,000 terms in order: 2^-16.
+    assert float(error) <= 2 * 2.0 ** -11 + 2.0 ** -22 + 2.0 ** -16
+
+
+@gpu_test
 def test_prefix_pages_without_tokens(kk):
     """Tables with pages that hold nothing yet, more in a row than a warp looks at once, at the start, inside and
     at the end; lanes and prefixes made of nothing else."""
