@@ -100,7 +100,7 @@ static_assert(kSliceRing <= 9, "the validity queue below holds eight slices");
 constexpr std::uint32_t kPoly = 1, kPolyOf = 4;
 
 constexpr float kRescale = 8.f;  // log2 growth of a row maximum that rescales O
-// Shared tokens' weights are 2^7 times as large as the maximum asks for: with that growth
+// Weights are 2^7 times as large as the maximum asks for: with that growth
 // they still stay below FP16's 2^16, and only those below 2^-21 of the largest one
 // fall among its subnormals.
 constexpr float kWeightLog2 = 7.f;
@@ -993,7 +993,7 @@ __device__ __forceinline__ void own_task(Args const& a, kk_prefix_item const& it
             float p[4];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                float const use = mrow[nt][h] == -INFINITY ? 0.f : mrow[nt][h];
+                float const use = mrow[nt][h] == -INFINITY ? 0.f : mrow[nt][h] - kWeightLog2;
                 p[h] = exp2_approx(x[h] - use);
                 p[2 + h] = exp2_approx(x[2 + h] - use);
                 lrow[nt][h] += p[h] + p[2 + h];
@@ -1040,7 +1040,7 @@ __device__ __forceinline__ void own_task(Args const& a, kk_prefix_item const& it
                     dst[part_chunk(row0 + qh, 4u * j + 2u + g / 4u) * 4u] = o[nt][j][2 + h];
                 }
                 if (g == 0) {
-                    a.part_ml[row0 + qh] = make_float2(mrow[nt][h], l);
+                    a.part_ml[row0 + qh] = make_float2(mrow[nt][h] - kWeightLog2, l);
                 }
             }
         }

@@ -397,12 +397,13 @@ def test_prefix_many_groups_and_lanes_without_one(kk):
 
 @gpu_test
 @pytest.mark.parametrize("score", [6.0, 9.0, 10.5, 11.0, 12.0, 13.0, 14.0])
-def test_prefix_one_token_outweighs_the_rest(kk, score):
+@pytest.mark.parametrize("group", [True, False], ids=["shared", "own"])
+def test_prefix_one_token_outweighs_the_rest(kk, score, group):
     """A first token with a score far above all others' (which are 0) and no value of its own: what is left
     of the result are the others' weights, e^-score each, and rounds no worse than any weight does."""
     pages = Pages(random.Random(21))
     tables = forks(pages, 4000, [0, 0])
-    s = Setup(kk, tables, pages, 8, 1, 22, sms=1)  # one part: the others stand next to it
+    s = Setup(kk, tables, pages, 8, 1, 22, sms=1, group=group)  # few parts: many of the others stand next to it
     for pool in (s.micro, s.extent):
         for part, value in ((0, 0.0), (1, 1.0)):
             x = pool[:, :, part]
