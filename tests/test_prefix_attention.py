@@ -426,6 +426,39 @@ def test_prefix_one_token_outweighs_the_rest(kk, score, group):
 
 
 @gpu_test
+@pytest.mark.parametrize("group", [True, False], ids=["shared", "own"])
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("token", [0, 77, 149, 160])
+def test_prefix_infinities_and_nan_among_the_keys(kk, group, value, token):
+    """One coordinate of one key: a score of +inf or NaN makes the row NaN, one of -inf weighs nothing; other KV
+    heads, and lanes that do not see the token, are as they would be."""
+    pages = Pages(random.Random(23))
+    tables = forks(pages, 150, [30, 0, 12])
+    s = Setup(kk, tables, pages, 12, 2, 24, group=group)
+    at = 0
+    for slot, _, n, kind in tables[0]:
+        if at <= token < at + n:
+            (s.extent if kind else s.micro)[slot, 1, 0, token - at, 1, 5] = value
+        at += n
+    s.run()
+    torch.cuda.synchronize()
+    assert kk.kernels()["device_status"](None) == 0
+    seen = 0
+    for b in range(3):
+        ref, _ = s.reference(1, b)
+        got = s.out[b, :12 * 64].double().view(12, 64)
+        lost = torch.isnan(ref)
+        seen += int(lost.sum())
+        assert bool((torch.isnan(got) == lost).all())
+        assert not bool(lost[:6].any())
+        # As in `reference`, with 2^8 for the largest sum of a score's terms (about 20 here; the rest leaves room
+        # for the FP32 sums) and 8 for the largest value.
+        over = (got - ref).abs() - (ref.abs() * 2.0 ** -11 + 2.0 ** -25 + 8 * (2.0 ** -8 + 2.0 ** -11))
+        assert float(over[~lost].max()) <= 0
+    assert seen > 0
+
+
+@gpu_test
 def test_prefix_pages_without_tokens(kk):
     """Tables with pages that hold nothing yet, more in a row than a warp looks at once, at the start, inside and
     at the end; lanes and prefixes made of nothing else."""
