@@ -24,23 +24,23 @@
 //  * warps 0-3 and 4-7 are two softmax groups, one thread per query row, each
 //    with its own O. Two row tiles: one group each, every K/V tile for both. One
 //    row tile: the groups take the token tiles in turn and join at the end.
-// P is rounded to FP16 for the second product (the row sums are not): its error,
-// 2^-12 of a weight on average, averages out to about that of the FP16 output.
-// The per-lane kernel adds the product of the low halves; here that second
-// product would be 64 columns wide and so at half of the tensor core's rate.
+// P goes into the second product as two FP16 values, what rounding leaves of it
+// being the second, as in the per-lane kernels: 22 bits of a weight. With the first
+// alone, a lane whose neighbours share its prefix would be less exact than one by
+// itself (64 lanes over each of two prefixes of 32,749 tokens: 57 us in place of
+// 67; results 1.4 times as far from 64 bits as FP16 rounding leaves them).
 // The running maximum is only raised, and O only rescaled, when a row's maximum
 // grows by more than 2^8 (P stays within FP16; the quotient is exact in either
 // case).
 // The exponentials, 16 per SM and clock, bound a K/V tile for 256 rows: 2,048
-// clocks, or 1,536 with a quarter of them on the FMA pipes. Measured: 2,500 clocks
-// (64 lanes over each of two prefixes of 32,749 tokens: 57 us); in the loop the
-// exponential unit is busy for 63 % of the time, issue slots for 59 %, the tensor
-// cores for 42 %; of a group's turn of 2,500 clocks 200 go by until it has seen its
-// scores, 150 until it holds them, 400 for the maximum, 1,450 for the weights, 300
-// until it looks for the next. Steps on the way, per such tile: 2.6 us with two groups that
+// clocks, or 1,536 with a quarter of them on the FMA pipes. Measured: 2,950 clocks
+// (64 lanes over each of two prefixes of 32,749 tokens: 67 us). Without the second
+// halves, of a group's turn of then 2,500 clocks 200 went by until it had seen its
+// scores, 150 until it held them, 400 for the maximum, 1,450 for the weights, 300
+// until it looked for the next. Steps on the way, per such tile: 2.6 us with two groups that
 // waited for each product (or four of half rows), while the products were issued
-// from a branch of one lane (see elect_lane); 1.9 us without that branch; 1.6 us
-// without the low halves; 1.4 us with the third S tile. No faster: four groups in
+// from a branch of one lane (see elect_lane); 1.9 us without that branch. Without the
+// second halves: 1.6 us; 1.4 us with the third S tile. No faster there: four groups in
 // turn over three S tiles (2.4 us, all three are then in use at once), 16 softmax
 // warps with a quarter of two rows a thread (1.7 us), an issuer for each group.
 //
@@ -86,7 +86,8 @@ constexpr std::uint32_t kTmemCols = 512;
 constexpr std::uint32_t kSTiles = 3;
 constexpr std::uint32_t kColS = 0;      // S tiles of 128 columns
 constexpr std::uint32_t kColO = 384;    // two O tiles of 64
-// P, two tokens to a column, replaces S from its start.
+// P, two tokens to a column, replaces S from its start; its low halves follow.
+constexpr std::uint32_t kColLow = kTile / 2;
 
 // A lane's own pages.
 constexpr std::uint32_t kSlice = 16;                       // tokens per step
@@ -95,14 +96,14 @@ constexpr std::uint32_t kSliceRing = kStages * kStageBytes / kOwnWarps / kSliceB
 static_assert(kSliceRing <= 9, "the validity queue below holds eight slices");
 
 // Of kPolyOf pairs of weights, kPoly are computed without the exponential unit.
-// Measured on 64 lanes over two prefixes of 32,749 tokens: 59.6 us with none,
-// 57.2 with one, 64.0 with two.
+// Measured on 64 lanes over two prefixes of 32,749 tokens: 68.1 us with none, 67.6
+// with one.
 constexpr std::uint32_t kPoly = 1, kPolyOf = 4;
 
 constexpr float kRescale = 8.f;  // log2 growth of a row maximum that rescales O
 // Weights are 2^7 times as large as the maximum asks for: with that growth
-// they still stay below FP16's 2^16, and only those below 2^-21 of the largest one
-// fall among its subnormals.
+// they still stay below FP16's 2^16, and what the two halves lose among its
+// subnormals is below 2^-32 of the largest one.
 constexpr float kWeightLog2 = 7.f;
 
 struct Args {
@@ -530,6 +531,7 @@ __device__ __forceinline__ void issue(kk_prefix_item const& item, std::uint8_t* 
             std::uint32_t const p = tmem + kColS + (q % kSTiles) * kTile + i * 8u;
             std::uint64_t const b = v_desc + i * 16u * (kRowBytes / 16u);
             mma_ts(elected, o, p, b, kIdescPV, q >= 2u || i != 0);
+            mma_ts(elected, o, p + kColLow, b, kIdescPV, 1u);
         }
         commit(elected, &sh->o_done[q % 2u]);
         if (!pair || q % 2u == 1u) {
@@ -668,25 +670,32 @@ __device__ __forceinline__ void soften(Args const& a, kk_prefix_item const& item
             std::uint64_t sum2[2] = {0, 0};
 #pragma unroll
             for (std::uint32_t c = 0; c < 4u; ++c) {
-                std::uint32_t p[16];
+                std::uint32_t p[16], low[16];
 #pragma unroll
                 for (std::uint32_t i = 0; i < 16u; ++i) {
                     std::uint32_t const at = c * 32u + 2u * i;
                     std::uint64_t const y = fma_f32x2(pack_f32x2(x[at], x[at + 1u]), scale2, shift2);
+                    std::uint64_t e;
                     float p0, p1;
                     if (i % kPolyOf < kPoly) {
-                        std::uint64_t const e = exp2_poly_f32x2(y);
+                        e = exp2_poly_f32x2(y);
                         unpack_f32x2(e, p0, p1);
-                        sum2[i % 2u] = add_f32x2(sum2[i % 2u], e);
                     } else {
                         unpack_f32x2(y, p0, p1);
                         p0 = exp2_approx(p0);
                         p1 = exp2_approx(p1);
-                        sum2[i % 2u] = add_f32x2(sum2[i % 2u], pack_f32x2(p0, p1));
+                        e = pack_f32x2(p0, p1);
                     }
+                    sum2[i % 2u] = add_f32x2(sum2[i % 2u], e);
                     p[i] = pack_half2(p0, p1);
+                    float l0, l1;  // what that leaves of the two: exact
+                    asm("{\n\t.reg .b16 a, b, m;\n\tmov.b32 {a, b}, %2;\n\tmov.b16 m, 0xBC00;\n\t"
+                        "fma.rn.f32.f16 %0, a, m, %3;\n\tfma.rn.f32.f16 %1, b, m, %4;\n\t}"
+                        : "=f"(l0), "=f"(l1) : "r"(p[i]), "f"(p0), "f"(p1));
+                    low[i] = pack_half2(l0, l1);
                 }
                 tmem_st16(s_col + c * 16u, p);
+                tmem_st16(s_col + kColLow + c * 16u, low);
             }
             float s0, s1;
             unpack_f32x2(add_f32x2(sum2[0], sum2[1]), s0, s1);

@@ -644,3 +644,73 @@ def test_prefix_reports_bad_pages_and_items(kk):
     s.run()
     s.check()
     assert torch.equal(s.out, good)
+
+
+@gpu_test
+@pytest.mark.parametrize("score", [1.25, 1.375, 2.75, 3.25, 5.5, 6.375, 6.875])
+@pytest.mark.parametrize("group", [True, False], ids=["shared", "own"])
+def test_prefix_weights_keep_more_bits_than_the_result(kk, score, group):
+    """All tokens but the first have the same score and value, so that their weights round alike; the value puts
+    the result right below 1, where half an FP16 step is 2^-12 of it. A weight of FP16's 11 bits (off by 2^-12.2
+    to 2^-11.1 at these scores) does not do."""
+    tokens = 1000
+    pages = Pages(random.Random(25))
+    s = Setup(kk, forks(pages, tokens, [0, 0]), pages, 8, 1, 26, sms=1, group=group)
+    for pool in (s.micro, s.extent):
+        for part in (0, 1):
+            x = pool[:, :, part]
+            x[~torch.isnan(x)] = 0.0
+    rest = (tokens - 1) * torch.exp(torch.tensor(-score, dtype=torch.float64))
+    share = float(rest / (1 + rest))
+    value = torch.tensor(1 / share).half()
+    while float(value) * share >= 1:
+        value = torch.nextafter(value, torch.zeros_like(value))
+    want = float(value) * share
+    assert 0.99 < want < 1
+    for pool in (s.micro, s.extent):
+        x = pool[:, :, 1]
+        x[~torch.isnan(x)] = float(value)
+    slot, _, _, kind = s.tables[0][0]
+    first = (s.extent if kind else s.micro)[slot, :, :, 0]
+    first.zero_()
+    first[:, 0, :, 0] = score / s.scale
+    s.q.zero_()
+    s.q.view(2, -1)[:, :512:64] = 1.0
+    s.run()
+    torch.cuda.synchronize()
+    assert kk.kernels()["device_status"](None) == 0
+    # Half a step of the result. Weights: 2^-18.5 each in the products and in the sum, their argument (7 + 16 at
+    # most in size, off by 2^-24 of that), 22 bits of them in the products. FP32 sums: two products for each of
+    # 63 steps of 16 tokens, 2^-23 a step; fewer additions in the sum of the weights.
+    bound = 2.0 ** -12 + 2 * 2.0 ** -18.5 + 2 * 2.0 ** -19.4 + 2.0 ** -21 + 2 * 63 * 2.0 ** -23 + 64 * 2.0 ** -24
+    assert float((s.out[:, :512].double() - want).abs().max()) <= bound
+
+
+@gpu_test
+@pytest.mark.parametrize("group", [True, False], ids=["shared", "own"])
+@pytest.mark.parametrize("page,prefix", [(8, 1), (8, 64), (8, 1333), (16, 700), (64, 3001), (8, 9000)])
+def test_prefix_every_token_counts_once(kk, group, page, prefix):
+    """Equal scores, and a value of one in dim t % 64 of token t: a dim of the result is the share of its tokens.
+    A token too few or too many moves one by 64 / tokens of itself, 2^-7.2 or more."""
+    rng = random.Random(page + prefix)
+    pages = Pages(rng, page)
+    tables = forks(pages, prefix, [0, 1, 77, 300], ragged=True)
+    s = Setup(kk, tables, pages, 16, 2, 27, group=group)
+    eye = torch.eye(64, dtype=torch.half, device="cuda")
+    for t in tables:
+        at = 0
+        for slot, _, n, kind in t:
+            ids = torch.arange(at, at + n, device="cuda") % 64
+            (s.extent if kind else s.micro)[slot, :, 1, :n] = eye[ids][None, :, None, :]
+            at += n
+    s.q.zero_()
+    s.run()
+    torch.cuda.synchronize()
+    assert kk.kernels()["device_status"](None) == 0
+    for b, t in enumerate(tables):
+        tokens = sum(e[2] for e in t)
+        want = torch.tensor([(tokens + 63 - d) // 64 for d in range(64)], dtype=torch.float64, device="cuda") / tokens
+        # Half an FP16 step; weights, in the products and in their sum; FP32 sums, 2^-24 a token: 2^-9.8 at most.
+        bound = want * (2.0 ** -11 + 2 * 2.0 ** -18.5 + tokens * 2.0 ** -24) + 2.0 ** -25
+        over = (s.out[b, :1024].double().view(16, 64) - want).abs() - bound
+        assert float(over.max()) <= 0
