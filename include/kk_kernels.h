@@ -204,8 +204,8 @@ KK_KAPI int kk_attention_set_variant(int variant);
  * of one prompt chunk) form a group; the group's pages are read once for all of
  * its query rows, each lane's remaining pages for that lane alone, and the
  * softmax parts are joined exactly. Same results as kk_paged_decode_attention
- * over the whole tables, up to FP32 rounding of the softmax sums and 2^-18.5 of
- * a shared token's weight (2^-32 of the row's largest one, if that is more).
+ * over the whole tables, up to FP32 rounding of the softmax sums and 2^-21 of a
+ * weight (2^-32 of the row's largest one, if that is more).
  *
  * Host side, once per step (the plan serves every layer):
  *   kk_prefix_groups finds the groups and cuts the shared pages off the lanes'

@@ -33,8 +33,9 @@
 // grows by more than 2^8 (P stays within FP16; the quotient is exact in either
 // case).
 // The exponentials, 16 per SM and clock, bound a K/V tile for 256 rows: 2,048
-// clocks, or 1,536 with a quarter of them on the FMA pipes. Measured: 2,950 clocks
-// (64 lanes over each of two prefixes of 32,749 tokens: 67 us). Without the second
+// clocks. Measured: 2,950 clocks (64 lanes over each of two prefixes of 32,749
+// tokens: 68 us); 67.6 us with a quarter of them by a polynomial on the FMA pipes, which
+// differ from the others by more than FP32 rounding. Without the second
 // halves, of a group's turn of then 2,500 clocks 200 went by until it had seen its
 // scores, 150 until it held them, 400 for the maximum, 1,450 for the weights, 300
 // until it looked for the next. Steps on the way, per such tile: 2.6 us with two groups that
@@ -94,11 +95,6 @@ constexpr std::uint32_t kSlice = 16;                       // tokens per step
 constexpr std::uint32_t kSliceBytes = 2 * kSlice * kRowBytes;
 constexpr std::uint32_t kSliceRing = kStages * kStageBytes / kOwnWarps / kSliceBytes;  // 6
 static_assert(kSliceRing <= 9, "the validity queue below holds eight slices");
-
-// Of kPolyOf pairs of weights, kPoly are computed without the exponential unit.
-// Measured on 64 lanes over two prefixes of 32,749 tokens: 68.1 us with none, 67.6
-// with one.
-constexpr std::uint32_t kPoly = 1, kPolyOf = 4;
 
 constexpr float kRescale = 8.f;  // log2 growth of a row maximum that rescales O
 // Weights are 2^7 times as large as the maximum asks for: with that growth
@@ -307,32 +303,6 @@ __device__ __forceinline__ float max_nan(float a, float b, float c)  // NaN if o
     float r;
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
-}
-
-// 2^x of two values on the FMA and ALU pipes, for the share of the weights that
-// the SM's 16 exponentials a clock leave waiting. x = n + f with n rounded to
-// nearest by adding 1.5 * 2^23, 2^f by a polynomial of degree 4 with the least
-// largest relative error on [-1/2, 1/2] (2.6e-6, found by the Remez exchange), n
-// added to the exponent. Below -126 it stays at 2^-126, which FP16 rounds to 0.
-__device__ __forceinline__ std::uint64_t exp2_poly_f32x2(std::uint64_t x)
-{
-    float x0, x1;
-    unpack_f32x2(x, x0, x1);
-    x = pack_f32x2(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
-    std::uint64_t const magic = pack_f32x2(12582912.f, 12582912.f);
-    std::uint64_t const minus = pack_f32x2(-12582912.f, -12582912.f);
-    std::uint64_t const n = add_f32x2(x, magic);
-    std::uint64_t const r = add_f32x2(n, minus);
-    std::uint64_t const f = fma_f32x2(r, pack_f32x2(-1.f, -1.f), x);
-    std::uint64_t p = fma_f32x2(f, pack_f32x2(0.0095701f, 0.0095701f), pack_f32x2(0.05591786f, 0.05591786f));
-    p = fma_f32x2(p, f, pack_f32x2(0.24024745f, 0.24024745f));
-    p = fma_f32x2(p, f, pack_f32x2(0.69312181f, 0.69312181f));
-    p = fma_f32x2(p, f, pack_f32x2(0.99999926f, 0.99999926f));
-    float p0, p1, n0, n1;
-    unpack_f32x2(p, p0, p1);
-    unpack_f32x2(n, n0, n1);
-    return pack_f32x2(__uint_as_float(__float_as_uint(p0) + (__float_as_uint(n0) << 23)),
-        __uint_as_float(__float_as_uint(p1) + (__float_as_uint(n1) << 23)));
 }
 
 __device__ __forceinline__ std::uint32_t pack_half2(float lo, float hi)
@@ -662,8 +632,7 @@ __device__ __forceinline__ void soften(Args const& a, kk_prefix_item const& item
                     }
                 }
             }
-            // A NaN or +inf among the scores makes the row NaN, whichever way its
-            // weight is computed.
+            // A NaN or +inf among the scores makes the row NaN.
             float const shift = !(mt < INFINITY) ? NAN : m == -INFINITY ? 0.f : kWeightLog2 - m;
             std::uint64_t const scale2 = pack_f32x2(a.scale_log2, a.scale_log2);
             std::uint64_t const shift2 = pack_f32x2(shift, shift);
@@ -675,18 +644,11 @@ __device__ __forceinline__ void soften(Args const& a, kk_prefix_item const& item
                 for (std::uint32_t i = 0; i < 16u; ++i) {
                     std::uint32_t const at = c * 32u + 2u * i;
                     std::uint64_t const y = fma_f32x2(pack_f32x2(x[at], x[at + 1u]), scale2, shift2);
-                    std::uint64_t e;
                     float p0, p1;
-                    if (i % kPolyOf < kPoly) {
-                        e = exp2_poly_f32x2(y);
-                        unpack_f32x2(e, p0, p1);
-                    } else {
-                        unpack_f32x2(y, p0, p1);
-                        p0 = exp2_approx(p0);
-                        p1 = exp2_approx(p1);
-                        e = pack_f32x2(p0, p1);
-                    }
-                    sum2[i % 2u] = add_f32x2(sum2[i % 2u], e);
+                    unpack_f32x2(y, p0, p1);
+                    p0 = exp2_approx(p0);
+                    p1 = exp2_approx(p1);
+                    sum2[i % 2u] = add_f32x2(sum2[i % 2u], pack_f32x2(p0, p1));
                     p[i] = pack_half2(p0, p1);
                     float l0, l1;  // what that leaves of the two: exact
                     asm("{\n\t.reg .b16 a, b, m;\n\tmov.b32 {a, b}, %2;\n\tmov.b16 m, 0xBC00;\n\t"

@@ -714,3 +714,38 @@ def test_prefix_every_token_counts_once(kk, group, page, prefix):
         bound = want * (2.0 ** -11 + 2 * 2.0 ** -18.5 + tokens * 2.0 ** -24) + 2.0 ** -25
         over = (s.out[b, :1024].double().view(16, 64) - want).abs() - bound
         assert float(over.max()) <= 0
+
+
+@gpu_test
+@pytest.mark.parametrize("score", [0.0, 0.25, 0.6, -1.1])
+@pytest.mark.parametrize("group", [True, False], ids=["shared", "own"])
+def test_prefix_equal_scores_have_equal_weights(kk, score, group):
+    """A value of +1000 is met by one of -1000 with the same score, wherever the two stand in a tile:
+    nothing is left of the sums but what the weights differ by."""
+    tokens = 1536
+    pages = Pages(random.Random(28))
+    s = Setup(kk, forks(pages, tokens, [0, 0]), pages, 8, 1, 29, sms=3, group=group)
+    at = 0
+    for slot, _, n, kind in s.tables[0]:
+        page = (s.extent if kind else s.micro)[slot]
+        t = torch.arange(at, at + n, device="cuda")
+        page[:, 0, :n] = 0.0
+        page[:, 0, :n, :, 0] = score / s.scale
+        page[:, 1, :n] = 0.0
+        for dim in range(64):  # +1000 for tokens t % 8 == a, -1000 for t % 8 == b
+            a, b = dim % 8, dim // 8
+            if a != b:
+                page[:, 1, :n, :, dim] = (1000.0 * ((t % 8 == a).half() - (t % 8 == b).half()))[None, :, None]
+        at += n
+    # One token outweighs them, so that their weights are no powers of two; it has no value.
+    slot, _, _, kind = s.tables[0][0]
+    first = (s.extent if kind else s.micro)[slot, :, :, :8]
+    first.zero_()
+    first[:, 0, 0, :, 0] = 2.0 / s.scale
+    s.q.zero_()
+    s.q.view(2, -1)[:, :512:64] = 1.0
+    s.run()
+    torch.cuda.synchronize()
+    assert kk.kernels()["device_status"](None) == 0
+    # A weight is off by 2^-21 at most, an eighth of the tokens have it, and half an FP16 step of what is left.
+    assert float(s.out[:, :512].abs().max()) <= 2 * 125 * 2.0 ** -21 * (1 + 2.0 ** -10)
