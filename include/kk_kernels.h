@@ -254,9 +254,12 @@ typedef struct kk_prefix_plan {
 /* Finds runs of at least max(2, min_lanes) consecutive lanes whose tables
  * begin with the same pages (slot, kind and valid tokens) for at least
  * min_tokens tokens, writes a group for each and moves the shared descriptors
- * out of those lanes (desc_offset, desc_count, token_count). A group takes
- * the pages that its first two lanes share, and the lanes that share all of
- * them. Returns the groups written (<= max_groups). */
+ * out of those lanes (desc_offset, desc_count, token_count). A group takes all
+ * pages that its lanes have in common. Of all ways to cut the lanes into runs
+ * the one with the largest sum of (lanes - 1) * (shared tokens + 1375) is taken
+ * (1375: what a group costs besides its tokens). Only neighbours are grouped: a
+ * caller puts lanes of one prefix next to each other (query_row leaves their
+ * rows where they are). Returns the groups written, the first max_groups. */
 KK_KAPI uint32_t kk_prefix_groups(const kk_page_desc* host_descs, kk_attn_lane* host_lanes,
     uint32_t num_lanes, uint32_t min_lanes, uint32_t min_tokens, kk_prefix_group* host_groups,
     uint32_t max_groups);

@@ -54,6 +54,8 @@
 
 #include <atomic>
 #include <cmath>
+#include <memory>
+#include <new>
 
 namespace kk {
 
@@ -1295,6 +1297,40 @@ std::uint32_t walkTiles(kk_page_desc const* descs, std::uint32_t begin, std::uin
     return closed + (n != 0 ? 1u : 0u);
 }
 
+// ---- grouping
+
+// A reader of pages costs its items' fixed part besides its tokens: as much as this
+// many tokens of a lane's own (kSharedNs / kOwnTokenNs). One group of many lanes is so
+// preferred to several that share a little more each.
+constexpr std::uint64_t kReaderTokens = 1375;
+
+struct Common {  // leading pages of two lanes that are the same
+    std::uint32_t pages;
+    std::uint64_t tokens;
+};
+
+struct Cut {  // between lanes at - 1 and at
+    std::uint32_t at;
+    std::uint32_t from;    // first lane of the group that ends here; at: none does
+    std::uint64_t gain;    // of the groups in front
+    std::uint32_t before;  // the cut where that choice begins,
+    std::uint32_t next;    // and on the way back the next one
+};
+
+Common commonPages(kk_page_desc const* descs, kk_attn_lane const& x, kk_attn_lane const& y)
+{
+    kk_page_desc const* const p = descs + x.desc_offset;
+    kk_page_desc const* const q = descs + y.desc_offset;
+    std::uint32_t const most = x.desc_count < y.desc_count ? x.desc_count : y.desc_count;
+    Common c{};
+    while (c.pages < most && p[c.pages].slot == q[c.pages].slot && p[c.pages].kind == q[c.pages].kind
+        && p[c.pages].valid_tokens == q[c.pages].valid_tokens) {
+        c.tokens += p[c.pages].valid_tokens;
+        ++c.pages;
+    }
+    return c;
+}
+
 bool headsServed(std::uint32_t q_heads, std::uint32_t kv_heads)
 {
     return kv_heads != 0 && q_heads != 0 && q_heads % kv_heads == 0 && q_heads / kv_heads <= 16u && q_heads <= 4096u;
@@ -1311,43 +1347,82 @@ extern "C" {
 uint32_t kk_prefix_groups(const kk_page_desc* descs, kk_attn_lane* lanes, uint32_t num_lanes, uint32_t min_lanes,
     uint32_t min_tokens, kk_prefix_group* groups, uint32_t max_groups)
 {
-    if (descs == nullptr || lanes == nullptr || groups == nullptr) {
+    using namespace kk;
+    min_lanes = min_lanes < 2u ? 2u : min_lanes;
+    if (descs == nullptr || lanes == nullptr || groups == nullptr || max_groups == 0 || num_lanes < min_lanes) {
         return 0;
     }
-    auto same = [](kk_page_desc const& x, kk_page_desc const& y) {
-        return x.slot == y.slot && x.kind == y.kind && x.valid_tokens == y.valid_tokens;
-    };
-    min_lanes = min_lanes < 2u ? 2u : min_lanes;
-    std::uint32_t found = 0;
-    for (std::uint32_t b = 0; found < max_groups && num_lanes - b >= min_lanes;) {
-        kk_page_desc const* const first = descs + lanes[b].desc_offset;
-        auto common = [&](kk_attn_lane const& other, std::uint32_t most) {
-            std::uint32_t n = 0;
-            while (n < most && n < other.desc_count && same(first[n], descs[other.desc_offset + n])) {
-                ++n;
-            }
-            return n;
-        };
-        std::uint32_t const pages = common(lanes[b + 1], lanes[b].desc_count);
-        std::uint64_t tokens = 0;
-        for (std::uint32_t n = 0; n < pages; ++n) {
-            tokens += first[n].valid_tokens;
+    // What lane b shares with lane b + 1. A run of lanes shares the least of its
+    // neighbours' common pages.
+    std::unique_ptr<Common[]> const common(new (std::nothrow) Common[num_lanes]);
+    std::unique_ptr<Cut[]> const cuts(new (std::nothrow) Cut[std::size_t(num_lanes) + 1u]);
+    if (common == nullptr || cuts == nullptr) {
+        return 0;  // every lane by itself: the same results
+    }
+    for (std::uint32_t b = 0; b + 1u < num_lanes; ++b) {
+        common[b] = commonPages(descs, lanes[b], lanes[b + 1u]);
+        if (common[b].tokens < min_tokens) {
+            common[b] = Common{};
         }
-        std::uint32_t end = b + 2u;
-        if (pages != 0 && tokens >= min_tokens) {
-            while (end < num_lanes && common(lanes[end], pages) == pages) {
-                ++end;
-            }
-        }
-        if (pages == 0 || tokens < min_tokens || end - b < min_lanes) {
-            ++b;
+    }
+    // The best sum of gains over the lanes in front of each cut. A group of two lanes
+    // or more that could end or begin inside a run of equal neighbours gains no
+    // less at one of the run's ends, so cuts inside are left out: 7 us for 32 lanes over
+    // 2,048 tokens, 154 us for 2 x 64 over 32,749 (81,715 descriptors), on the host.
+    std::uint32_t n = 0;
+    cuts[n++] = Cut{0, 0, 0, 0, 0};
+    for (std::uint32_t at = 1; at <= num_lanes; ++at) {
+        bool const inside = min_lanes == 2u && at > 1u && at + 1u < num_lanes
+            && common[at - 1u].pages == common[at - 2u].pages && common[at - 1u].pages == common[at].pages;
+        if (inside) {
             continue;
         }
-        std::uint32_t const count = static_cast<std::uint32_t>(tokens);
-        groups[found++] = kk_prefix_group{lanes[b].desc_offset, pages, count, b, end - b, 0, 0, 0};
-        for (; b < end; ++b) {
-            lanes[b].desc_offset += pages;
-            lanes[b].desc_count -= pages;
+        Cut& cut = cuts[n];
+        cut = Cut{at, at, cuts[n - 1u].gain, n - 1u, 0};  // no group ends here
+        std::uint64_t least = ~std::uint64_t{0};  // tokens that the lanes from `from` on share
+        for (std::uint32_t k = n; k-- > 0;) {
+            std::uint32_t const from = cuts[k].at, to = cuts[k + 1u].at;
+            if (to != at && common[to - 1u].tokens < least) {
+                least = common[to - 1u].tokens;  // across the cut
+            }
+            if (to - from > 1u && common[from].tokens < least) {
+                least = common[from].tokens;  // between the cuts: all equal
+            }
+            if (least == 0) {
+                break;
+            }
+            if (at - from >= min_lanes) {
+                std::uint64_t const gain = cuts[k].gain + (at - from - 1u) * (least + kReaderTokens);
+                if (gain >= cut.gain) {
+                    cut = Cut{at, from, gain, k, 0};
+                }
+            }
+        }
+        ++n;
+    }
+    // Back along the choices, then forward over the groups.
+    std::uint32_t next = 0;
+    for (std::uint32_t k = n - 1u; k != 0;) {
+        std::uint32_t const before = cuts[k].before;
+        cuts[k].next = next;
+        next = k;
+        k = before;
+    }
+    std::uint32_t found = 0;
+    for (std::uint32_t k = next; k != 0 && found < max_groups; k = cuts[k].next) {
+        std::uint32_t const from = cuts[k].from, end = cuts[k].at;
+        if (from == end) {
+            continue;
+        }
+        Common least = common[from];
+        for (std::uint32_t b = from; b + 1u < end; ++b) {
+            least = common[b].pages < least.pages ? common[b] : least;
+        }
+        std::uint32_t const count = static_cast<std::uint32_t>(least.tokens);
+        groups[found++] = kk_prefix_group{lanes[from].desc_offset, least.pages, count, from, end - from, 0, 0, 0};
+        for (std::uint32_t b = from; b < end; ++b) {
+            lanes[b].desc_offset += least.pages;
+            lanes[b].desc_count -= least.pages;
             lanes[b].token_count -= lanes[b].token_count < count ? lanes[b].token_count : count;
         }
     }

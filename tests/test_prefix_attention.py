@@ -102,6 +102,94 @@ def test_groups_differ_by_valid_tokens_and_stop_at_room(kk):
         assert kk.kernels()["prefix_groups"](descs, lanes, empty, 2, 1, groups, 1) == 0
 
 
+def own_tokens(lanes, n):
+    return sum(lanes[i].token_count for i in range(n))
+
+
+@pytest.mark.parametrize("at", [0, 5, 31, 63])
+def test_groups_with_a_short_lane_among_long_ones(kk, at):
+    """A lane that holds only the first page of what the others share does not cut their sharing down to it."""
+    pages = Pages(random.Random(30))
+    shared = pages.table(64) + pages.table(4096, 64)
+    tables = [shared[:1] if i == at else shared + pages.table(i, 4160) for i in range(64)]
+    assert shared[0][2] == 64
+    descs, lanes, nd = pack(kk, tables)
+    groups, n = find(kk, descs, lanes, 64, min_tokens=64)
+    assert n == (2 if at in (5, 31) else 1)
+    for g in range(n):
+        assert groups[g].token_count == 4160 and groups[g].desc_count == len(shared)
+    assert sum(groups[g].lane_count for g in range(n)) == 63
+    assert own_tokens(lanes, 64) == sum(i for i in range(64) if i != at) + 64
+
+
+def test_groups_of_pairs_that_share_a_little_more(kk):
+    """Lanes that share a long prompt, every two of them some tokens behind it: the prompt is read once."""
+    pages = Pages(random.Random(31))
+    prompt = pages.table(2000)
+    tables = []
+    for _ in range(16):
+        more = prompt + pages.table(100, 2000)
+        tables += [more + pages.table(3, 2100), more + pages.table(9, 2100)]
+    descs, lanes, nd = pack(kk, tables)
+    groups, n = find(kk, descs, lanes, 32)
+    assert n == 1 and (groups[0].lane_begin, groups[0].lane_count, groups[0].token_count) == (0, 32, 2000)
+    # Pairs that share much more than the prompt stand alone.
+    tables = []
+    for _ in range(4):
+        more = prompt[:4] + pages.table(9000, 256)
+        tables += [more + pages.table(3, 9256), more + pages.table(9, 9256)]
+    descs, lanes, nd = pack(kk, tables)
+    assert find(kk, descs, lanes, 8)[1] == 4
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_groups_have_the_largest_gain(kk, seed):
+    """Against every way to cut the lanes into runs. A run of n lanes gains (n - 1) x (shared tokens + 1375)."""
+    rng = random.Random(seed)
+    pages = Pages(rng)
+    n = rng.randint(1, 9)
+    pieces = [[pages.table(rng.choice([1, 8, 64, 200, 3000])) for _ in range(2)] for _ in range(4)]
+    tables = []
+    for _ in range(n):
+        t = []
+        for p_ in pieces[:rng.randint(0, 4)]:
+            t += p_[int(rng.random() < 0.2)]
+        tables.append(t + (pages.table(rng.randint(1, 70)) if rng.random() < 0.7 else []))
+    if rng.random() < 0.5:
+        tables.sort(key=lambda t: [e[:1] + e[2:] for e in t])
+    min_lanes, min_tokens = rng.choice([0, 2, 2, 3, 4]), rng.choice([0, 1, 64, 250])
+
+    def shared(b, e):
+        count = 0
+        while all(count < len(t) for t in tables[b:e]) and len({t[count][:1] + t[count][2:] for t in tables[b:e]}) == 1:
+            count += 1
+        return count, sum(x[2] for x in tables[b][:count])
+
+    def gain(b, e):
+        tokens = shared(b, e)[1]
+        return (e - b - 1) * (tokens + 1375) if e - b >= max(2, min_lanes) and tokens >= max(1, min_tokens) else 0
+
+    best = [0] * (n + 1)
+    for e in range(1, n + 1):
+        best[e] = max(best[b] + gain(b, e) for b in range(e))
+    descs, lanes, nd = pack(kk, tables)
+    before = [(lanes[b].desc_offset, lanes[b].desc_count, lanes[b].token_count) for b in range(n)]
+    groups, ng = find(kk, descs, lanes, n, min_lanes, min_tokens)
+    end, total = 0, 0
+    grouped = {}
+    for g in groups[:ng]:
+        assert g.lane_begin >= end and gain(g.lane_begin, g.lane_begin + g.lane_count) > 0
+        end = g.lane_begin + g.lane_count
+        assert (g.desc_count, g.token_count) == shared(g.lane_begin, end) and g.desc_offset == before[g.lane_begin][0]
+        total += gain(g.lane_begin, end)
+        grouped.update({b: g for b in range(g.lane_begin, end)})
+    assert end <= n and total == best[n]
+    for b in range(n):
+        cut = (grouped[b].desc_count, grouped[b].token_count) if b in grouped else (0, 0)
+        assert (lanes[b].desc_offset, lanes[b].desc_count, lanes[b].token_count) == (
+            before[b][0] + cut[0], before[b][1] - cut[0], before[b][2] - cut[1])
+
+
 def tile_fill(entries):
     """128-token tiles of a run as the kernel fills them: 16 groups of 8 tokens, pages whole."""
     tiles, n = 0, 0
