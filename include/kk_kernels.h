@@ -259,7 +259,10 @@ typedef struct kk_prefix_plan {
  * the one with the largest sum of (lanes - 1) * (shared tokens + 1375) is taken
  * (1375: what a group costs besides its tokens). Only neighbours are grouped: a
  * caller puts lanes of one prefix next to each other (query_row leaves their
- * rows where they are). Returns the groups written, the first max_groups. */
+ * rows where they are). A small group can cost more than it saves (36 pairs that
+ * share 300 tokens, 4 KV heads: 19.0 us, 14.6 without groups; 30 times four lanes
+ * that share 3,000, 8 KV heads: 90 us, 174 without): min_lanes and min_tokens
+ * leave those out. Returns the groups written, the first max_groups. */
 KK_KAPI uint32_t kk_prefix_groups(const kk_page_desc* host_descs, kk_attn_lane* host_lanes,
     uint32_t num_lanes, uint32_t min_lanes, uint32_t min_tokens, kk_prefix_group* host_groups,
     uint32_t max_groups);

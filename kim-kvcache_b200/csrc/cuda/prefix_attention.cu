@@ -1485,7 +1485,8 @@ int kk_prefix_attention_plan(const kk_page_desc* descs, uint32_t num_descs, kk_a
         g.part_row = walkTiles(descs, g.desc_offset, g.desc_offset + g.desc_count, [](std::uint32_t, std::uint32_t) {});
         longest = std::fmax(longest, kSharedNs + g.part_row * tileNs(g));
     }
-    // The shortest time in which num_sms blocks, one to an SM, can do the work.
+    // The shortest time in which num_sms blocks, one to an SM, can do the work, or as
+    // many rounds of them as take the least time in all.
     auto partsIn = [&](kk_prefix_group const& g, double ns) {
         double const most = std::fmax(1., std::floor((ns - kSharedNs) / tileNs(g)));
         return static_cast<std::uint32_t>(std::ceil(g.part_row / most));
@@ -1521,14 +1522,31 @@ int kk_prefix_attention_plan(const kk_page_desc* descs, uint32_t num_descs, kk_a
         }
         return blocks;
     };
-    double lo = 0., hi = std::fmax(longest, kOwnNs + kTaskNs + kTaskTokenNs * 0x1p32);
-    for (int i = 0; i < 48; ++i) {
-        double const mid = 0.5 * (lo + hi);
-        bool const done = mid >= kSharedNs && mid >= kOwnNs + kTaskNs
-            && sharedBlocksIn(mid) + ownBlocksIn(mid) <= num_sms;
-        (done ? hi : lo) = mid;
+    double const most_time = std::fmax(longest, kOwnNs + kTaskNs + kTaskTokenNs * 0x1p32);
+    // One block per prefix, KV head and pair of row tiles, and one for the lanes' own
+    // pages, are the fewest. Up to half of the SMs, the others are enough for own pages
+    // (8 KV heads, 4 lanes with up to 1,000 tokens behind each prefix of 300, in one
+    // round and in the best number: 10 prefixes 29.6 and 21.2 us, 16 prefixes 133 and 32).
+    double const fewest = sharedBlocksIn(most_time) + (own_tokens != 0 ? 1. : 0.);
+    double time = 0., waves = 0.;
+    double const first_waves = std::fmax(1., std::ceil(fewest / num_sms));
+    for (double w = first_waves; w < first_waves + 8.; ++w) {
+        double lo = 0., hi = most_time;
+        for (int i = 0; i < 48; ++i) {
+            double const mid = 0.5 * (lo + hi);
+            bool const done = mid >= kSharedNs && mid >= kOwnNs + kTaskNs
+                && sharedBlocksIn(mid) + ownBlocksIn(mid) <= w * num_sms;
+            (done ? hi : lo) = mid;
+        }
+        if (waves != 0. && w * hi >= waves * time) {
+            break;
+        }
+        time = hi;
+        waves = w;
+        if (2. * fewest <= num_sms) {
+            break;
+        }
     }
-    double const time = hi;
     std::uint32_t count = 0;
     std::uint64_t part_rows = 0;
     auto put = [&](kk_prefix_item const& item) {
@@ -1577,9 +1595,8 @@ int kk_prefix_attention_plan(const kk_page_desc* descs, uint32_t num_descs, kk_a
         // What the prefixes leave of the SMs, and no less than the plan set aside.
         std::uint32_t blocks = static_cast<std::uint32_t>(std::fmin(ownBlocksIn(time), 1e6));
         blocks = blocks < 1u ? 1u : blocks;
-        if (count < num_sms && blocks < num_sms - count) {
-            blocks = num_sms - count;
-        }
+        double const left = std::fmin(waves * num_sms, 1e6) - count;
+        blocks = blocks < left ? static_cast<std::uint32_t>(left) : blocks;
         // The shortest items that those blocks take in as many rounds.
         double const longest_task = taskTokensIn(time);
         double const room = std::floor(roundsIn(time, tasksOf(longest_task))) * blocks * kOwnWarps;

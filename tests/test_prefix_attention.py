@@ -276,6 +276,29 @@ def test_plan_covers_every_page_once(kk, seed, sms):
         assert rc == 0 and small.num_items == plan.num_items and few[3].owner == 77
 
 
+@pytest.mark.parametrize("groups,lanes,prefix,own,hkv", [
+    (16, 4, 300, 1000, 8), (18, 2, 64, 1000, 8), (19, 2, 64, 1000, 8), (32, 4, 300, 1000, 8), (36, 2, 300, 500, 4),
+    (40, 2, 300, 500, 4), (128, 2, 64, 64, 8), (1, 4096, 256, 30, 4), (9, 3, 3000, 700, 8),
+])
+def test_plan_spreads_own_pages_beside_many_prefixes(kk, groups, lanes, prefix, own, hkv):
+    """As many prefixes, times KV heads and row tiles, as there are SMs and more: what the lanes have of their own
+    is spread over many thread blocks all the same."""
+    rng = random.Random(groups)
+    pages = Pages(rng)
+    tables = []
+    for _ in range(groups):
+        tables += forks(pages, prefix, [rng.randint(0, own) for _ in range(lanes)])
+    descs, lane_array, nd = pack(kk, tables)
+    group_array, ng = find(kk, descs, lane_array, len(tables))
+    assert ng == groups
+    rc, items, plan = plan_for(kk, descs, nd, lane_array, len(tables), group_array, ng, 4 * hkv, hkv)
+    assert rc == 0 and plan.num_items <= 65536
+    flat = [e for t in tables for e in t]
+    work = [sum(flat[e][2] for e in range(it.desc_begin, it.desc_end)) for it in items[plan.num_shared:plan.num_items]]
+    blocks = [sum(work[i:i + plan.tasks_per_cta]) for i in range(0, len(work), plan.tasks_per_cta)]
+    assert max(blocks) <= 4 * sum(work) / 148 + 8 * 64
+
+
 def test_plan_refuses(kk):
     pages = Pages(random.Random(3))
     shared = pages.table(100)
