@@ -504,7 +504,8 @@ KK_KAPI int kk_gemm(const kk_gemm_desc* desc, void* stream);
  * array and mask rows outside the masks are reported by kk_device_status; the
  * row's history or biases are then left out, respectively the row is masked
  * entirely. Bias ids that descend within a row are reported too; what that row
- * gets of its biases is not specified. Arrays are 4-byte aligned. */
+ * gets of its biases is not specified. Arrays are 4-byte aligned; history_size
+ * and bias_size are at most 2^32 - 256. */
 #define KK_NO_TOKEN 0xffffffffu
 #define KK_NO_MASK 0xffffffffu
 typedef struct kk_logits_desc {

@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 4) logits_process_kernel(const __gri
                 __syncthreads();
             }
             std::uint32_t const listed = penal ? s_listed : 0u;
-            if (listed + (b1 - b0) > kListed && run > kFewBlocks) {
+            if ((listed > kListed || b1 - b0 > kListed - listed) && run > kFewBlocks) {
                 run = kFewBlocks;
                 __syncthreads();
                 if (tid == 0) {
@@ -658,6 +658,12 @@ extern "C" int kk_logits_process(const kk_logits_desc* d, void* stream)
         return KK_EINVAL;
     }
     if (d->bias_offsets != nullptr && d->bias_size != 0 && (d->bias_tokens == nullptr || d->bias_values == nullptr)) {
+        return KK_EINVAL;
+    }
+    // A 32-bit index passes the end of its list by a step of the block.
+    constexpr std::uint64_t kMaxEntries = (std::uint64_t(1) << 32) - kThreads;
+    if ((a.d.history_offsets != nullptr && d->history_size > kMaxEntries)
+        || (d->bias_offsets != nullptr && d->bias_size > kMaxEntries)) {
         return KK_EINVAL;
     }
     if (d->mask != nullptr && d->mask_stride < (d->vocab + 31u) / 32u) {

@@ -46,6 +46,20 @@ def test_logits_refuses(kk, change):
     assert kk.kernels()["logits_process"](C.byref(d), None) == kk.KK_EINVAL
 
 
+@pytest.mark.parametrize("change", [
+    dict(bias_offsets=16, bias_tokens=16, bias_values=16, bias_size=(1 << 32) - 255),
+    dict(bias_offsets=16, bias_tokens=16, bias_values=16, bias_size=1 << 40),
+    dict(repetition=16, history_offsets=16, history=16, history_size=(1 << 32) - 255),
+    dict(repetition=16, history_offsets=16, history=16, history_size=1 << 33),
+], ids=str)
+def test_logits_refuses_lists_that_32_bit_indices_cannot_step_over(kk, change):
+    """A row's list that ends within a step of 2^32 would be walked for ever."""
+    d = valid_desc(kk)
+    for name, value in change.items():
+        setattr(d, name, value)
+    assert kk.kernels()["logits_process"](C.byref(d), None) == kk.KK_EINVAL
+
+
 def test_logits_without_rows_launches_nothing(kk):
     d = valid_desc(kk)
     d.rows = 0
