@@ -15,6 +15,7 @@
 #include "launch.cuh"
 
 #include <cmath>
+#include <limits>
 
 namespace kk {
 
@@ -507,13 +508,16 @@ int kk_kv_append_rope(const kk_kv_append_desc* d, void* stream)
         a.cos_sin = reinterpret_cast<float2 const*>(d->cos_sin);
         a.table_positions = d->table_positions;
         if (a.cos_sin == nullptr) {
-            // theta^(-2i / rotary_dim) by repeated products of one power. The
-            // i-th is off by i roundings of 2^-53 of a value that shrinks
-            // with i: below 2^-53 turns per position, 2^-21 at the farthest.
-            double const ratio = std::pow(static_cast<double>(d->theta), -2.0 / d->rotary_dim);
-            double turns = 0.15915494309189535;  // 1 / (2 pi)
+            // theta^(-2i / rotary_dim) by repeated products of one power, with 64
+            // bits of mantissa: after i of them, and with the power's own rounding, off by
+            // less than 2i + 1 roundings of 2^-64 of a value below 2^-2.6. For 128 powers
+            // that is 2^-58.6 turns per position and, with the cut to 2^-64, 2^-26.5 at the
+            // farthest, 7e-8 rad. (With 53 bits it was 2.5e-5 rad for a theta near 1.)
+            static_assert(std::numeric_limits<long double>::digits >= 64, "");
+            long double const ratio = powl(d->theta, -2.0L / d->rotary_dim);
+            long double turns = 0.159154943091895335768883763372514362L;  // 1 / (2 pi)
             for (std::uint32_t i = 0; i < d->rotary_dim / 2; ++i, turns *= ratio) {
-                a.turns[i] = static_cast<std::uint64_t>((turns - std::floor(turns)) * 0x1p64);
+                a.turns[i] = static_cast<std::uint64_t>(turns * 0x1p64L);
             }
         }
     }

@@ -322,3 +322,37 @@ def test_append_behind_32_bit_offsets(kk):
     assert_rounded(got, rotate_ref(turned, positions, 64, 10000.0), np.concatenate([ab, ab], -1))
     assert np.array_equal(page_now[1, 1, [63, 0, 5]], x[:, hq + hkv:])
     assert (page_now[0] == 7).all() and (np.delete(page_now[1], [63, 0, 5], 1) == 7).all()
+
+
+@gpu_test
+@pytest.mark.parametrize("theta", [1.0, 1.0001, 1.5, 5.0, 37.0, 10000.0, 1e6, 3e38])
+@pytest.mark.parametrize("rotary", [64, 128, 256])
+def test_append_angles_of_any_theta(kk, theta, rotary):
+    """The farthest positions, where an error of a power of theta counts 2^32 times. The pairs are (1, 0) and
+    (0, 1): the results are cosines and sines, and those near zero tell the angle to 4e-6 rad in FP16."""
+    theta = float(np.float32(theta))
+    rows, dim, half = 1024, 256, rotary // 2
+    rng = np.random.RandomState(rotary)
+    positions = rng.randint((1 << 32) - 100000, 1 << 32, rows, dtype=np.uint64).astype(np.uint32)
+    positions[0] = 0xFFFFFFFF
+    x = np.zeros((rows, 4, dim), np.float16)  # two query heads, a key and a value
+    x[:, 0, :half] = x[:, 1, half:rotary] = x[:, 2, :half] = 1.0
+    micro = torch.zeros(rows // 64, 1, 2, 64, 1, dim, dtype=torch.half, device="cuda")
+    slots = to_device_bytes((kk.KvSlot * rows)(*[kk.KvSlot(r // 64, r % 64, 0, 1) for r in range(rows)]))
+    d_x, d_pos = torch.from_numpy(x.reshape(rows, -1)).cuda(), torch.from_numpy(positions.view(np.int32)).cuda()
+    out = torch.zeros(rows, 2 * dim, dtype=torch.half, device="cuda")
+    d = kk.KvAppendDesc()
+    d.pools = kk.KvPools(p(micro), 0, rows // 64, 0, 1, 1, dim, 64)
+    d.layer, d.rows, d.q_heads, d.rotary_dim, d.theta = 0, rows, 2, rotary, theta
+    d.slots, d.positions = p(slots), p(d_pos)
+    d.query, d.key, d.value = p(d_x), p(d_x) + 4 * dim, p(d_x) + 6 * dim
+    d.query_stride = d.key_stride = d.value_stride = 4 * dim
+    d.query_out, d.query_out_stride = p(out), 2 * dim
+    torch.cuda.synchronize()
+    assert kk.kernels()["kv_append_rope"](C.byref(d), None) == 0
+    torch.cuda.synchronize()
+    assert kk.kernels()["device_status"](None) == 0
+    got = np.concatenate([out.cpu().numpy().reshape(rows, 2, dim), micro[:, 0, 0].cpu().numpy().reshape(rows, 1, dim)], 1)
+    size = np.zeros(got.shape)
+    size[..., :rotary] = 1.0
+    assert_rounded(got, rotate_ref(x[:, :3], positions, rotary, theta), size)
