@@ -437,7 +437,9 @@ __global__ void __launch_bounds__(kThreads, 4) logits_process_kernel(const __gri
                     if (owned(v) && bias_next != v) {
                         std::uint32_t const at = place_of(v);
                         if (at / kBlock - block0 < block1 - block0) {
-                            if ((s_touched[at / 32u] >> (at % 32u) & 1u) != 0) {
+                            std::uint32_t const volatile& marks = s_touched[at / 32u];
+                            if ((marks >> (at % 32u) & 1u) != 0) {
+                                __threadfence_block();  // where ids descend, see below
                                 float& y = s_value[word_of(at)];
                                 y = __fadd_rn(y, bias_value);
                             } else {
@@ -445,6 +447,9 @@ __global__ void __launch_bounds__(kThreads, 4) logits_process_kernel(const __gri
                                 if (place < kListed) {  // as ever, unless ids descend
                                     s_value[place] = __fadd_rn(bias_logit, bias_value);
                                     set_word(at, place);
+                                    // Where ids descend, another thread may have the same
+                                    // token: it sees the mark only with the place.
+                                    __threadfence_block();
                                     atomicOr(&s_touched[at / 32u], 1u << (at % 32u));
                                 }
                             }

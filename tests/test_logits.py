@@ -360,3 +360,30 @@ def test_logits_behind_32_bit_offsets(kk):
         host[r, host[r].argmax()] += np.float32(-100.0)
         assert np.array_equal(x[r * stride:r * stride + vocab].cpu().numpy(), host[r])
     assert np.array_equal(tokens.cpu().numpy(), host.argmax(1))
+
+
+@gpu_test
+@pytest.mark.parametrize("history", [0, 70000], ids=["alone", "with_history"])
+@pytest.mark.parametrize("ids", ["shuffled", "one_id_and_others"])
+def test_logits_descending_bias_ids_stay_in_their_row(kk, history, ids):
+    """Biases out of order, ids again and again: reported, and whatever the row gets of them, tokens without a
+    bias and the other rows are as they would be."""
+    vocab = 20000
+    c = Case(3, vocab, seed=30)
+    if history:
+        c.with_history([50, history, 0], prompts=[0, 100, 0])
+    c.with_bias([300, 0, 70])
+    n = 6000
+    named = c.rng.randint(0, 3000, n).astype(np.uint32)
+    if ids == "one_id_and_others":
+        named[::2] = 1234
+    c.bias[1] = (named, np.ones(n, np.float32))
+    for _ in range(3):
+        out, tokens, _ = c.call(kk)
+        assert kk.kernels()["device_status"](None) == 3
+        x, want = c.expect()
+        free = np.setdiff1d(np.arange(vocab), named)
+        assert np.array_equal(out[[0, 2]], x[[0, 2]]) and np.array_equal(tokens[[0, 2]], want[[0, 2]])
+        assert np.array_equal(out[1, free], x[1, free])
+        assert np.isfinite(out[1]).all()
+        assert tokens[1] == int(np.argmax(out[1]))
