@@ -1161,6 +1161,7 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(const __grid_
         && (ln.item_count == 0 || own + std::uint64_t(ln.item_count - 1u) * q_heads < a.plan.part_rows);
     if (!fits) {
         report(kErrBadArgument);
+        pdl_wait();  // this launch must not end before the one that writes the partials
         return;
     }
     pdl_launch_dependents();

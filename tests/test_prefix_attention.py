@@ -860,3 +860,37 @@ def test_prefix_equal_scores_have_equal_weights(kk, score, group):
     assert kk.kernels()["device_status"](None) == 0
     # A weight is off by 2^-21 at most, an eighth of the tokens have it, and half an FP16 step of what is left.
     assert float(s.out[:, :512].abs().max()) <= 2 * 125 * 2.0 ** -21 * (1 + 2.0 ** -10)
+
+
+@gpu_test
+def test_prefix_lanes_that_do_not_fit_the_plan(kk):
+    """Lanes whose partial rows lie outside the plan's are reported and their rows left as they were; the calls
+    behind, which use the same workspace, are not touched by them."""
+    pages = Pages(random.Random(32))
+    tables = forks(pages, 3000, [20, 500, 64, 7])
+    s = Setup(kk, tables, pages, 32, 4, 33)
+    s.run()
+    s.check()
+    good = s.out.clone()
+    lanes = (kk.AttnLane * 4)(*s.lanes[:4])
+    for b in range(4):
+        lanes[b].item_offset = 0xFFFFFFF0
+    dev = to_device_bytes(lanes)
+    for b in range(4):
+        lanes[b].item_offset, lanes[b].item_count = s.lanes[b].item_offset, 0xFFFFFFFF
+    more = to_device_bytes(lanes)
+    for bad in (dev, more):
+        s.out[:, :2048] = 3.0
+        s.desc.lanes = p(bad)
+        s.run()
+        torch.cuda.synchronize()
+        assert kk.kernels()["device_status"](None) == 3
+        assert bool((s.out[:, :2048] == 3.0).all())
+        for _ in range(5):
+            s.desc.lanes = p(bad)
+            s.run()
+            s.desc.lanes = p(s.dev[1])
+            s.run()
+        torch.cuda.synchronize()
+        assert kk.kernels()["device_status"](None) == 3
+        assert torch.equal(s.out, good)
