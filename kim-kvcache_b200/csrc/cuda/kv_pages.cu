@@ -435,6 +435,7 @@ __device__ __forceinline__ std::uint64_t mix64(std::uint64_t x)
 
 __global__ void fill_fp16_kernel(__half* data, std::uint64_t count, std::uint64_t seed, float scale)
 {
+    pdl_wait();
     for (std::uint64_t i = blockIdx.x * std::uint64_t(blockDim.x) + threadIdx.x; i < count;
          i += std::uint64_t(gridDim.x) * blockDim.x) {
         std::uint64_t const h = mix64(seed * 0x100000001b3ull + i);

@@ -356,3 +356,36 @@ def test_append_angles_of_any_theta(kk, theta, rotary):
     size = np.zeros(got.shape)
     size[..., :rotary] = 1.0
     assert_rounded(got, rotate_ref(x[:, :3], positions, rotary, theta), size)
+
+
+@gpu_test
+def test_append_inputs_filled_again_as_a_programmatic_dependent(kk):
+    """kk_fill_fp16 launched ahead of the append's end waits for it before it writes over the append's inputs."""
+    rows, hq, hkv, D = 16384, 32, 8, 128
+    width = (hq + 2 * hkv) * D
+    K = kk.kernels()
+    micro = torch.zeros(rows // 64, 1, 2, 64, hkv, D, dtype=torch.half, device="cuda")
+    slots = to_device_bytes((kk.KvSlot * rows)(*[kk.KvSlot(r // 64, r % 64, 0, 1) for r in range(rows)]))
+    pos = torch.arange(rows, dtype=torch.int32, device="cuda")
+    x, out = torch.empty(rows, width, dtype=torch.half, device="cuda"), torch.empty(rows, hq * D, dtype=torch.half, device="cuda")
+    d = kk.KvAppendDesc()
+    d.pools = kk.KvPools(p(micro), 0, rows // 64, 0, 1, hkv, D, 64)
+    d.layer, d.rows, d.q_heads, d.rotary_dim, d.theta = 0, rows, hq, D, 10000.0
+    d.slots, d.positions = p(slots), p(pos)
+    d.query, d.key, d.value = (p(x) + 2 * D * n for n in (0, hq, hq + hkv))
+    d.query_stride = d.key_stride = d.value_stride = width
+    d.query_out, d.query_out_stride = p(out), hq * D
+    torch.cuda.synchronize()
+    kept = []
+    for pdl in (0, 1, 1, 1):
+        assert K["fill_fp16"](p(x), x.numel(), 1, 1.0, None) == 0
+        torch.cuda.synchronize()
+        K["set_pdl"](pdl)
+        assert K["kv_append_rope"](C.byref(d), None) == 0
+        assert K["fill_fp16"](p(x), x.numel(), 2, 1.0, None) == 0
+        K["set_pdl"](0)
+        torch.cuda.synchronize()
+        assert K["device_status"](None) == 0
+        kept.append((out.clone(), micro.clone()))
+    for a, b in kept[1:]:
+        assert torch.equal(a, kept[0][0]) and torch.equal(b, kept[0][1])
