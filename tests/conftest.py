@@ -28,6 +28,27 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "slow: long-running CPU test")
 
 
+# Refusals that are tested with made-up addresses: where a device is present, a
+# refusal that got lost would launch a kernel on them.
+MADE_UP_ADDRESSES = {
+    "test_append_refuses", "test_append_without_rows_launches_nothing", "test_logits_refuses",
+    "test_logits_refuses_lists_that_32_bit_indices_cannot_step_over", "test_logits_without_rows_launches_nothing",
+    "test_attention_refuses", "test_attention_without_lanes_launches_nothing",
+}
+
+
+def device_present() -> bool:
+    import torch
+    return torch.cuda.is_available()
+
+
+def pytest_collection_modifyitems(config, items):
+    named = [i for i in items if getattr(i, "originalname", None) in MADE_UP_ADDRESSES]
+    if named and device_present():
+        for item in named:
+            item.add_marker(pytest.mark.skip(reason="made-up addresses: runs where there is no device"))
+
+
 def load_kk():
     spec = importlib.util.spec_from_file_location(
         "kim_kvcache_b200", ROOT / "kim-kvcache_b200" / "__init__.py")
