@@ -499,7 +499,8 @@ KK_KAPI int kk_gemm(const kk_gemm_desc* desc, void* stream);
  * a row that leaves nothing else gets KK_NO_TOKEN. Results do not depend on
  * the order in which threads run.
  * Strides are in elements; rows may start at any multiple of 4 bytes. vocab is
- * at most 400,000 where a history or biases are given, 10 million otherwise.
+ * at most 400,000 where a history or biases are given, 10 million with a mask
+ * alone, 2^30 with none of them.
  * Ids outside the vocabulary are ignored. Offsets that decrease or pass their
  * array and mask rows outside the masks are reported by kk_device_status; the
  * row's history or biases are then left out, respectively the row is masked

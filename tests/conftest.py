@@ -33,6 +33,7 @@ def pytest_configure(config):
 MADE_UP_ADDRESSES = {
     "test_append_refuses", "test_append_without_rows_launches_nothing", "test_logits_refuses",
     "test_logits_refuses_lists_that_32_bit_indices_cannot_step_over", "test_logits_without_rows_launches_nothing",
+    "test_logits_refuses_vocabularies_beyond_their_limits",
     "test_attention_refuses", "test_attention_without_lanes_launches_nothing",
 }
 

@@ -387,3 +387,67 @@ def test_logits_descending_bias_ids_stay_in_their_row(kk, history, ids):
         assert np.array_equal(out[1, free], x[1, free])
         assert np.isfinite(out[1]).all()
         assert tokens[1] == int(np.argmax(out[1]))
+
+
+@gpu_test
+@pytest.mark.parametrize("vocab,masked", [(400000, False), (400001, True), (400003, False), (9999999, True), (10000000, True),
+                                          (10000001, False), (40000003, False)], ids=str)
+@pytest.mark.parametrize("in_place", [False, True])
+def test_logits_vocabularies_beyond_the_listed_tokens(kk, vocab, masked, in_place):
+    """Without history and biases nothing is counted: the vocabulary may be larger, up to 10 million with a mask."""
+    c = Case(2 if vocab < 10 ** 6 else 1, vocab, seed=vocab % 1000, stride=vocab + 3)
+    c.logits[0, [vocab - 1, vocab // 2]] = 100.0
+    if masked:
+        c.with_mask(0.5)
+        c.mask[0, vocab // 2 // 32] &= ~np.uint32(1 << (vocab // 2 % 32))
+        c.mask[0, (vocab - 1) // 32] |= np.uint32(1 << ((vocab - 1) % 32))
+    c.check(kk, in_place=in_place, offset=1)
+    assert c.expect()[1][0] == (vocab - 1 if masked else vocab // 2)
+
+
+@pytest.mark.parametrize("vocab,kw", [
+    (400001, dict(bias_offsets=16)), (400001, dict(repetition=16, history_offsets=16)),
+    (10000001, dict(mask=16, mask_stride=1 << 20, num_masks=1)), ((1 << 30) + 1, {}),
+], ids=str)
+def test_logits_refuses_vocabularies_beyond_their_limits(kk, vocab, kw):
+    d = valid_desc(kk)
+    d.vocab, d.logits_stride, d.out_stride = vocab, 1 << 31, 1 << 31
+    for name, value in kw.items():
+        setattr(d, name, value)
+    assert kk.kernels()["logits_process"](C.byref(d), None) == kk.KK_EINVAL
+
+
+@gpu_test
+def test_logits_calls_that_overlap_on_two_streams(kk):
+    """Everything is built first; then calls are launched alternately on two streams, with nothing in between."""
+    built = []
+    for seed, (rows, vocab, history) in enumerate(((20, 20011, 900), (64, 32000, 4000))):
+        c = Case(rows, vocab, seed=40 + seed).with_history([history] * rows, prompts=[100] * rows).with_bias([9] * rows)
+        c.with_mask(0.9)
+        up = lambda a, t: torch.from_numpy(np.ascontiguousarray(a).view(t)).cuda()  # noqa: E731
+        ends = lambda lists: np.cumsum([0] + [len(a) for a in lists]).astype(np.uint32)  # noqa: E731
+        arrays = dict(logits=up(c.logits, np.float32), history=up(np.concatenate(c.history), np.int32),
+                      history_offsets=up(ends(c.history), np.int32), prompt_counts=up(c.prompts, np.int32),
+                      repetition=up(c.factors[0], np.float32), presence=up(c.factors[1], np.float32),
+                      frequency=up(c.factors[2], np.float32), bias_tokens=up(np.concatenate([b[0] for b in c.bias]), np.int32),
+                      bias_values=up(np.concatenate([b[1] for b in c.bias]), np.float32),
+                      bias_offsets=up(ends([b[0] for b in c.bias]), np.int32), mask=up(c.mask, np.int32),
+                      out=torch.zeros(rows, vocab, device="cuda"), tokens=torch.zeros(rows, dtype=torch.int32, device="cuda"))
+        d = kk.LogitsDesc()
+        for name, t in arrays.items():
+            setattr(d, name, p(t))
+        d.logits_stride = d.out_stride = d.vocab = vocab
+        d.rows, d.history_size, d.bias_size = rows, len(arrays["history"]), len(arrays["bias_tokens"])
+        d.mask_stride, d.num_masks = c.mask.shape[1], rows
+        built.append((c, d, arrays, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    call = kk.kernels()["logits_process"]
+    for _ in range(20):
+        for c, d, arrays, stream in built:
+            assert call(C.byref(d), stream.cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert kk.kernels()["device_status"](None) == 0
+    for c, d, arrays, _ in built:
+        x, want = c.expect()
+        assert np.array_equal(arrays["out"].cpu().numpy(), x)
+        assert np.array_equal(arrays["tokens"].cpu().numpy(), want)
