@@ -389,3 +389,39 @@ def test_append_inputs_filled_again_as_a_programmatic_dependent(kk):
         kept.append((out.clone(), micro.clone()))
     for a, b in kept[1:]:
         assert torch.equal(a, kept[0][0]) and torch.equal(b, kept[0][1])
+
+
+@gpu_test
+def test_append_calls_that_overlap_on_two_streams(kk):
+    """Two batches into pages of their own, launched alternately on two streams with nothing in between."""
+    K, D, built = kk.kernels(), 64, []
+    for seed, (rows, hq, hkv) in enumerate(((3000, 8, 2), (700, 32, 4))):
+        rng = np.random.RandomState(50 + seed)
+        x = (rng.randn(rows, hq + 2 * hkv, D) * 2).astype(np.float16)
+        positions = rng.randint(0, 1 << 20, rows).astype(np.uint32)
+        arrays = [torch.from_numpy(x.reshape(rows, -1)).cuda(), torch.from_numpy(positions.view(np.int32)).cuda(),
+                  to_device_bytes((kk.KvSlot * rows)(*[kk.KvSlot(r // 64, r % 64, 0, 1) for r in range(rows)])),
+                  torch.zeros(rows, hq * D, dtype=torch.half, device="cuda"),
+                  torch.zeros(rows // 64 + 1, 1, 2, 64, hkv, D, dtype=torch.half, device="cuda")]
+        d = kk.KvAppendDesc()
+        d.pools = kk.KvPools(p(arrays[4]), 0, rows // 64 + 1, 0, 1, hkv, D, 64)
+        d.layer, d.rows, d.q_heads, d.rotary_dim, d.theta = 0, rows, hq, D, 10000.0
+        d.slots, d.positions = p(arrays[2]), p(arrays[1])
+        d.query, d.key, d.value = (p(arrays[0]) + 2 * D * n for n in (0, hq, hq + hkv))
+        d.query_stride = d.key_stride = d.value_stride = (hq + 2 * hkv) * D
+        d.query_out, d.query_out_stride = p(arrays[3]), hq * D
+        built.append((x, positions, hq, hkv, arrays, d, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for *_, d, stream in built:
+            assert K["kv_append_rope"](C.byref(d), stream.cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert K["device_status"](None) == 0
+    for x, positions, hq, hkv, arrays, _, _ in built:
+        rows = len(x)
+        page = arrays[4][:, 0].cpu().numpy().transpose(1, 0, 2, 3, 4).reshape(2, -1, hkv, D)[:, :rows]
+        got = np.concatenate([arrays[3].cpu().numpy().reshape(rows, hq, D), page[0]], 1)
+        turned = x[:, :hq + hkv]
+        ab = np.abs(turned[..., :32].astype(float)) + np.abs(turned[..., 32:].astype(float))
+        assert_rounded(got, rotate_ref(turned, positions, D, 10000.0), np.concatenate([ab, ab], -1))
+        assert np.array_equal(page[1], x[:, hq + hkv:])

@@ -276,6 +276,27 @@ def test_plan_covers_every_page_once(kk, seed, sms):
         assert rc == 0 and small.num_items == plan.num_items and few[3].owner == 77
 
 
+def test_plan_refuses_descriptors_behind_the_end(kk):
+    """Every lane and the group reach to some last descriptor: one fewer is refused, as many are enough."""
+    pages = Pages(random.Random(34))
+    shared = pages.table(100)
+    for tails in ([0, 0, 0], [5, 0, 9], [0, 70, 0], [3, 3, 3]):
+        tables = [shared + pages.table(n, 100) for n in tails]
+        for grouped in (True, False):
+            descs, lanes, nd = pack(kk, tables)
+            groups, ng = find(kk, descs, lanes, 3) if grouped else ((kk.PrefixGroup * 1)(), 0)
+            assert ng == int(grouped)
+            assert plan_for(kk, descs, nd, lanes, 3, groups, ng, 32, 4)[0] == 0
+            assert plan_for(kk, descs, nd - 1, lanes, 3, groups, ng, 32, 4)[0] == kk.KK_EINVAL
+            if not grouped:
+                continue
+            # The lanes' own tables inside, the group's run one too long.
+            groups[0].desc_offset, groups[0].desc_count = nd - 2, 3
+            assert plan_for(kk, descs, nd, lanes, 3, groups, 1, 32, 4)[0] == kk.KK_EINVAL
+            groups[0].desc_count = 2
+            assert plan_for(kk, descs, nd, lanes, 3, groups, 1, 32, 4)[0] == 0
+
+
 @pytest.mark.parametrize("groups,lanes,prefix,own,hkv", [
     (16, 4, 300, 1000, 8), (18, 2, 64, 1000, 8), (19, 2, 64, 1000, 8), (32, 4, 300, 1000, 8), (36, 2, 300, 500, 4),
     (40, 2, 300, 500, 4), (128, 2, 64, 64, 8), (1, 4096, 256, 30, 4), (9, 3, 3000, 700, 8),
