@@ -103,6 +103,9 @@ constexpr float kRescale = 8.f;  // log2 growth of a row maximum that rescales O
 // they still stay below FP16's 2^16, and what the two halves lose among its
 // subnormals is below 2^-32 of the largest one.
 constexpr float kWeightLog2 = 7.f;
+// A score in log2 units from which on the rounding of kWeightLog2 less that score
+// shows (2^-6 here; from 2^23 on weights leave FP16's range).
+constexpr float kFarLog2 = 0x1p18f;
 
 struct Args {
     __half const* micro;
@@ -125,6 +128,8 @@ struct Args {
     std::uint64_t query_stride;
     std::uint64_t output_stride;
     float scale_log2;
+    float far_score;            // scores of kFarLog2 and kRescale in log2 units
+    float rescale_score;
     float* part_o;              // [part_rows][64]
     float2* part_ml;            // [part_rows] maximum (log2 units), sum
 };
@@ -571,7 +576,9 @@ __device__ __forceinline__ void soften(Args const& a, kk_prefix_item const& item
         return __all_sync(0xffffffffu, wait_or_abort(bar, phase & 1u, abort)) != 0;
     };
     std::uint32_t const turns = turns_of(item);
-    float m = -INFINITY;  // reference maximum of the row, log2 units
+    float ref = -INFINITY;  // reference maximum of the row's scores
+    float limit = -INFINITY;  // a score above this one moves the reference
+    float shift = 0.f;      // weights are 2^(score * scale_log2 + shift)
     float l = 0.f;
     bool ok = true;
     for (std::uint32_t q = t; q < turns; q += 2u) {
@@ -608,13 +615,25 @@ __device__ __forceinline__ void soften(Args const& a, kk_prefix_item const& item
             for (std::uint32_t i = 0; i < kTile; i += 2u) {
                 top[i / 2u % 4u] = max_nan(top[i / 2u % 4u], x[i], x[i + 1u]);
             }
-            float const mt = max_nan(max_nan(top[0], top[1], top[2]), top[3], top[3]) * a.scale_log2;
-            bool const grow = mt > m + kRescale || m == -INFINITY;
-            if (__any_sync(0xffffffffu, grow)) {
-                float const now = grow ? mt : m;
-                float const alpha = m == -INFINITY ? 1.f : exp2_approx(m - now);
-                m = now;
+            float const highest = max_nan(max_nan(top[0], top[1], top[2]), top[3], top[3]);
+            if (__any_sync(0xffffffffu, highest > limit)) {
+                bool const grow = (highest - ref) * a.scale_log2 > kRescale || ref == -INFINITY;
+                float const now = grow ? highest : ref;
+                float const alpha = ref == -INFINITY ? 1.f : exp2_approx((ref - now) * a.scale_log2);
+                ref = now;
                 l *= alpha;
+                // So far out that kWeightLog2 less the reference would lose the weight: the
+                // reference is taken off the scores, of every tile from here on.
+                bool const far = fabsf(ref) > a.far_score && fabsf(ref) < INFINITY;
+                limit = far ? -INFINITY : ref + a.rescale_score;
+                shift = ref == -INFINITY ? 0.f : far ? kWeightLog2 : kWeightLog2 - ref * a.scale_log2;
+                if (__any_sync(0xffffffffu, far)) {
+                    float const less = far ? ref : 0.f;
+#pragma unroll
+                    for (std::uint32_t i = 0; i < kTile; ++i) {
+                        x[i] -= less;
+                    }
+                }
                 if (k != 0) {
                     // Once the last product into O is done.
                     ok = wait(&sh->o_done[t], k - 1u);
@@ -635,9 +654,9 @@ __device__ __forceinline__ void soften(Args const& a, kk_prefix_item const& item
                 }
             }
             // A NaN or +inf among the scores makes the row NaN.
-            float const shift = !(mt < INFINITY) ? NAN : m == -INFINITY ? 0.f : kWeightLog2 - m;
+            float const use = highest < INFINITY ? shift : NAN;
             std::uint64_t const scale2 = pack_f32x2(a.scale_log2, a.scale_log2);
-            std::uint64_t const shift2 = pack_f32x2(shift, shift);
+            std::uint64_t const shift2 = pack_f32x2(use, use);
             std::uint64_t sum2[2] = {0, 0};
 #pragma unroll
             for (std::uint32_t c = 0; c < 4u; ++c) {
@@ -674,6 +693,7 @@ __device__ __forceinline__ void soften(Args const& a, kk_prefix_item const& item
     }
     ok = ok && wait(&sh->o_full, 0);
     tc_fence_after();
+    float m = ref * a.scale_log2;
     // One row tile: the second group's O joins the first's through the ring,
     // which nothing uses any more.
     constexpr std::uint32_t kStride = kHeadDim + 3;  // odd: rows fall into different banks
@@ -944,7 +964,7 @@ __device__ __forceinline__ void own_task(Args const& a, kk_prefix_item const& it
             // As in the shared items, the reference follows the maximum only when
             // that has grown by 2^8: a vote in place of two reductions a slice.
             float const top0 = fmaxf(x[0], x[2]), top1 = fmaxf(x[1], x[3]);
-            if (__any_sync(0xffffffffu, top0 > mrow[nt][0] + kRescale || top1 > mrow[nt][1] + kRescale
+            if (__any_sync(0xffffffffu, top0 - mrow[nt][0] > kRescale || top1 - mrow[nt][1] > kRescale
                     || mrow[nt][0] == -INFINITY)) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -966,9 +986,9 @@ __device__ __forceinline__ void own_task(Args const& a, kk_prefix_item const& it
             float p[4];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                float const use = mrow[nt][h] == -INFINITY ? 0.f : mrow[nt][h] - kWeightLog2;
-                p[h] = exp2_approx(x[h] - use);
-                p[2 + h] = exp2_approx(x[2 + h] - use);
+                float const use = mrow[nt][h] == -INFINITY ? 0.f : mrow[nt][h];
+                p[h] = exp2_approx(x[h] - use + kWeightLog2);
+                p[2 + h] = exp2_approx(x[2 + h] - use + kWeightLog2);
                 lrow[nt][h] += p[h] + p[2 + h];
             }
             float hp[4];
@@ -1727,6 +1747,8 @@ int kk_prefix_attention(const kk_prefix_attn_desc* d, void* stream)
     a.query_stride = d->query_stride;
     a.output_stride = d->output_stride;
     a.scale_log2 = d->scale * 1.4426950408889634f;
+    a.far_score = kFarLog2 / a.scale_log2;
+    a.rescale_score = kRescale / a.scale_log2;
     a.part_o = static_cast<float*>(d->workspace);
     a.part_ml = reinterpret_cast<float2*>(a.part_o + d->plan.part_rows * kHeadDim);
     cudaStream_t const s = static_cast<cudaStream_t>(stream);

@@ -915,3 +915,45 @@ def test_prefix_lanes_that_do_not_fit_the_plan(kk):
         torch.cuda.synchronize()
         assert kk.kernels()["device_status"](None) == 3
         assert torch.equal(s.out, good)
+
+
+@gpu_test
+@pytest.mark.parametrize("group", [True, False], ids=["shared", "own"])
+@pytest.mark.parametrize("size", [30.0, 300.0, 1000.0, 4000.0, 10000.0, 20000.0])
+def test_prefix_scores_of_any_size(kk, group, size):
+    """Scores up to 10^10, where FP32 tells neighbours further apart than FP16's whole range of weights: a row's
+    result is the value of its highest token, wherever that one leads by more than the scores are off."""
+    pages = Pages(random.Random(35))
+    s = Setup(kk, forks(pages, 1500, [0, 40, 300]), pages, 8, 2, 36, sms=3, group=group, q_scale=size)
+    for pool in (s.micro, s.extent):
+        pool[:, :, 0] *= min(size, 10000.0)
+    s.q.clamp_(-60000.0, 60000.0)
+    s.run()
+    torch.cuda.synchronize()
+    assert kk.kernels()["device_status"](None) == 0
+    told = 0
+    for b, t in enumerate(s.tables):
+        k, v = torch.cat([(s.extent if kind else s.micro)[slot, 1, :, :n] for slot, _, n, kind in t], 1).double()
+        q = s.q[b, :512].double().view(2, -1, 64)
+        score = torch.einsum("hgd,thd->hgt", q, k) * s.scale
+        top, at = score.topk(2, -1)
+        terms = torch.einsum("hgd,thd->hgt", q.abs(), k.abs()).amax(-1) * s.scale
+        # 64 products in FP32, 2^-23 a step at most; as much again for the factor and the maximum. A lead of 40 more
+        # leaves e^-40 of the others.
+        lead = top[..., 0] - top[..., 1] > 40 + 2 * 2.0 ** -17 * terms
+        want = v[at[..., 0], torch.arange(2, device="cuda")[:, None]]  # [head, query head, 64]
+        got = s.out[b, :512].double().view(2, -1, 64)
+        assert bool(torch.isfinite(got).all()), f"lane {b}"
+        assert bool(((got - want).abs() <= want.abs() * 2.0 ** -11 + 2.0 ** -25)[lead].all()), f"lane {b}"
+        told += int(lead.sum())
+    assert told >= 12  # of 24
+
+
+@gpu_test
+def test_prefix_lanes_without_any_tokens(kk):
+    """Nothing to plan: the rows are zeros."""
+    pages = Pages(random.Random(37))
+    s = Setup(kk, [[], [], []], pages, 32, 4, 38)
+    assert s.plan.num_items == 0
+    s.run()
+    s.check()
