@@ -530,6 +530,8 @@ int kk_kv_append_rope(const kk_kv_append_desc* d, void* stream)
     // per CTA; 4,999 rows of 16 + 2 heads of 128, half rotated: 12.8 us, 14.6 with
     // four). More rows: many waves, of four rows per CTA (16,384 rows of 32 + 8
     // heads of 128: 72.5 us, 74.4 with five, 76.8 with seven, before loads went around L1).
+    // On the two sides of the step, 5,920 and 5,921 rows: 29.3 and 27.9 us for 32 + 8
+    // heads of 128, 16.1 and 17.4 for 32 + 4 of 64, 15.0 and 16.9 for 16 + 2 of 128 half rotated.
     a.rows_per_cta = d->rows <= kAppendWave * kAppendMaxRows ? (d->rows - 1u) / kAppendWave + 1u : 4u;
     a.q_heads = d->q_heads;
     a.kv_heads = d->pools.kv_heads;

@@ -1285,10 +1285,14 @@ cudaError_t allowSharedMemory()
 
 // ---- planning -------------------------------------------------------------------
 
-// Measured times of a thread block, in nanoseconds, from which the plan deals
-// the SMs out between the prefixes and the lanes' own pages. (Those of own items
-// with the cost of joining their parts: shorter items than these give are no
-// faster, 13.9 us in place of 13.0 for 32 lanes with up to 1,024 tokens.)
+// Times of a thread block, in nanoseconds, from which the plan deals the SMs out
+// between the prefixes and the lanes' own pages. (Those of own items with the cost of
+// joining their parts: shorter items than these give are no faster, 13.9 us in
+// place of 13.0 for 32 lanes with up to 1,024 tokens.) Tiles measure 1,650 and 1,100
+// where nothing else runs. With those two plans are no better, and worse where own
+// pages, which then take longer than these say, get fewer SMs for it: 8 prefixes of
+// 10,000 tokens, 8 KV heads, 8 lanes each with up to 1,000 of their own: 142 us in
+// place of 119.
 constexpr double kSharedNs = 5500.;     // a shared item without its tiles
 constexpr double kTilePairNs = 1450.;   // a 128-token tile for two row tiles
 constexpr double kTileSingleNs = 750.;  // for one
