@@ -27,8 +27,8 @@
 // P goes into the second product as two FP16 values, what rounding leaves of it
 // being the second, as in the per-lane kernels: 22 bits of a weight. With the first
 // alone, a lane whose neighbours share its prefix would be less exact than one by
-// itself (64 lanes over each of two prefixes of 32,749 tokens: 57 us in place of
-// 67; results 1.4 times as far from 64 bits as FP16 rounding leaves them).
+// itself (64 lanes over each of two prefixes of 32,749 tokens: 57 us in place of 68,
+// results 1.4 times as far from 64 bits as FP16 rounding leaves them).
 // The running maximum is only raised, and O only rescaled, when a row's maximum
 // grows by more than 2^8 (P stays within FP16; the quotient is exact in either
 // case).
