@@ -957,3 +957,38 @@ def test_prefix_lanes_without_any_tokens(kk):
     assert s.plan.num_items == 0
     s.run()
     s.check()
+
+
+@gpu_test
+@pytest.mark.parametrize("groups,lanes,prefix,own,hq,hkv", [
+    (40, 3, 300, 200, 32, 8),     # more prefixes times KV heads than SMs: rounds of blocks
+    (19, 2, 64, 1000, 8, 8),
+    (1, 600, 200, 20, 16, 1),     # 75 tiles of query rows over one prefix
+    (1, 700, 130, 9, 28, 4),
+])
+def test_prefix_many_groups_and_many_rows(kk, groups, lanes, prefix, own, hq, hkv):
+    rng = random.Random(groups + lanes)
+    pages = Pages(rng)
+    tables = []
+    for _ in range(groups):
+        tables += forks(pages, prefix, [rng.randint(0, own) for _ in range(lanes)])
+    s = Setup(kk, tables, pages, hq, hkv, 39)
+    assert s.ng == groups
+    s.run()
+    s.check()
+
+
+@gpu_test
+def test_prefix_short_lanes_among_long_ones(kk):
+    """Lanes that share more with some neighbours than with others, in every order."""
+    rng = random.Random(40)
+    pages = Pages(rng)
+    a, b, c = pages.table(64), pages.table(2000, 64), pages.table(500, 64)
+    tables = []
+    for kind in "saabbsacasbb":
+        head = {"s": a, "a": a + b, "b": a + c, "c": a + b + c}[kind]
+        tables.append(head + pages.table(rng.choice([0, 1, 40]), sum(e[2] for e in head)))
+    s = Setup(kk, tables, pages, 32, 4, 41)
+    assert s.ng >= 1
+    s.run()
+    s.check()
