@@ -1416,6 +1416,13 @@ uint32_t kk_prefix_groups(const kk_page_desc* descs, kk_attn_lane* lanes, uint32
             if (least == 0) {
                 break;
             }
+            // A group from here or further in front could end at `to` instead; no choice up to
+            // there is worth more than that cut's gain, and the lanes behind it add no
+            // more than this. Where that is too little the search is over. (2,048 lanes whose
+            // neighbours all share different runs: 0.6 ms, 8.6 without this.)
+            if (min_lanes == 2u && to != at && cuts[k + 1u].gain + (at - to) * (least + kReaderTokens) < cut.gain) {
+                break;
+            }
             if (at - from >= min_lanes) {
                 std::uint64_t const gain = cuts[k].gain + (at - from - 1u) * (least + kReaderTokens);
                 if (gain >= cut.gain) {
